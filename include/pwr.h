@@ -34,7 +34,7 @@ extern "C" {
 #define PWR_HEATMAP_SUM 1     /* model.py:86-90 */
 
 /* ABI version of this header; pwr_abi_version() must return the same number. */
-#define PWR_ABI_VERSION 7   /* 7 (round 6): pwr_conv_dgrad_fold_stats_pair; 6 (round 6): pwr_norm_bwd_apply_from_partial, pwr_norm_bwd_params_from_partial, pwr_norm_bwd_params_group, pwr_norm_finalize_partial_pair, pwr_engine_pack_beside_forward, pwr_norm_apply, pwr_norm_stats_fused_src, pwr_nchw_to_nhwc_pad_pair; 5 (round 5): pwr_conv_fwd_nchw_pair, the order field of the pack records and the tag bit of a fragment-order pack; 4 (round 4): pwr_conv_dgrad_stats_pair, pwr_conv_wgrad_pair, pwr_engine_wait_segment, pwr_resblock_bwd_small_x, pwr_norm_bwd_from_partial_pair, pwr_conv_fwd_stats mode 1; 3 (round 3): experiment entry points removed, debugging aids moved to pwr_debug.h */
+#define PWR_ABI_VERSION 8   /* 8: pwr_likelihood_*, pwr_orthogonalize, pwr_muon_*, pwr_engine_logits_offset, pwr_engine_logit_grad; 7 (round 6): pwr_conv_dgrad_fold_stats_pair; 6 (round 6): pwr_norm_bwd_apply_from_partial, pwr_norm_bwd_params_from_partial, pwr_norm_bwd_params_group, pwr_norm_finalize_partial_pair, pwr_engine_pack_beside_forward, pwr_norm_apply, pwr_norm_stats_fused_src, pwr_nchw_to_nhwc_pad_pair; 5 (round 5): pwr_conv_fwd_nchw_pair, the order field of the pack records and the tag bit of a fragment-order pack; 4 (round 4): pwr_conv_dgrad_stats_pair, pwr_conv_wgrad_pair, pwr_engine_wait_segment, pwr_resblock_bwd_small_x, pwr_norm_bwd_from_partial_pair, pwr_conv_fwd_stats mode 1; 3 (round 3): experiment entry points removed, debugging aids moved to pwr_debug.h */
 int pwr_abi_version(void);
 
 /* ---------------------------------------------------------------------------------------------
@@ -352,6 +352,11 @@ int pwr_engine_pack_beside_forward(void* engine);
 int pwr_engine_forward(void* engine, const float* img, const float* label, const float* mask, void* const* outs,
                        int training, void* stream);
 long long pwr_engine_generation(void* engine);
+/* Where in the arena the logits of a stage's heat maps are after pwr_engine_forward (fp32 [B,J,P,P]; SIZE_MAX: no such stage), and a gradient with
+ * respect to them (gz [B,J,P,P]) and to the stage's w (gw [J], softmax only) that the NEXT pwr_engine_backward of that stage adds to what it computes;
+ * either may be NULL.  A forward drops what no backward has taken. */
+size_t pwr_engine_logits_offset(void* engine, int stage);
+int pwr_engine_logit_grad(void* engine, int stage, const float* gz, const float* gw);
 /* gouts: HOST array of 3*stage device pointers with the gradients of the outputs (NULL = zero).  Runs backward
  * segment `seg`; segment 0 first zeroes grads[0:n_grad_floats].  Parameter gradients are written (not
  * accumulated) into the bound flat gradient buffer, in the layout of the parameters. */
@@ -376,6 +381,52 @@ int pwr_adamw_step(float* p, const float* g, float* m, float* v, long long n, fl
                    float weight_decay, int step, float grad_scale, void* stream);
 int pwr_sgd_step(float* p, const float* g, float* buf, long long n, float lr, float momentum, float weight_decay, int first,
                  float grad_scale, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Log likelihood of a heat map's pixel, with the map's entropy and its most likely pixels, and the gradient of the first two.  The distribution
+ * is the decoder's (model.py:83-85), p = softmax_i(s), s_i = w[j] z_i, over the pixels a mask allows.
+ * z: `rows` rows of V values of `dtype`, ldz apart (any alignment); row r belongs to joint r % J.  w: [J] fp32 or NULL (1).  mask: fp32 rows of V
+ * (0 = not allowed), mask row r / mask_rows (J: one per sample, 1: one per row) or NULL.  index: [rows] or NULL; < 0: no pixel given, log
+ * likelihood 0 and no gradient; >= V: NaN.
+ * logp, entropy: [rows] fp32, either may be NULL.  stats: [rows][2] fp32 for the backward pass, or NULL.  top_logp [rows][K] fp32, top_index
+ * [rows][K]: the K most likely pixels in order, equal ones by the lowest index; K <= 32, 0 = none (both may be NULL).
+ * A pixel with s = -inf has no probability, like a masked one.  A row without any: log likelihood -inf, entropy 0, no alternatives (-inf, -1), zero
+ * gradient.  What is masked may hold NaN or inf; a NaN or +inf that is allowed makes its row's results NaN.
+ * PWR_EUNSUPPORTED: K > 32, or K > 4096 / pieces for a row of V > 16384 values, which is worked on in ceil(V / 16384) pieces or more.
+ * ------------------------------------------------------------------------------------------- */
+size_t pwr_likelihood_workspace_bytes(long long rows, int V, int K);
+int pwr_likelihood_fwd(const void* z, long long ldz, const float* w, int J, const float* mask, int mask_rows, const long long* index,
+                       float* logp, float* entropy, float* stats, float* top_logp, long long* top_index, long long rows, int V, int K, int dtype,
+                       void* workspace, size_t workspace_bytes, void* stream);
+/* gz [rows][V] of `dtype` (contiguous) = the gradient of sum(glogp logp) + sum(gentropy entropy) with respect to z; glogp / gentropy [rows] or NULL
+ * (zero); stats, entropy: from the forward pass.  gw [J] or NULL: the gradient with respect to w (rows a multiple of J); the workspace is for gw only. */
+size_t pwr_likelihood_bwd_workspace_bytes(long long rows, int V);
+int pwr_likelihood_bwd(const void* z, long long ldz, const float* w, int J, const float* mask, int mask_rows, const long long* index,
+                       const float* stats, const float* entropy, const float* glogp, const float* gentropy, void* gz, float* gw, long long rows,
+                       int V, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Newton-Schulz orthogonalisation: X = G / (|G|_F + eps); `steps` times A = X X^T, X = a X + (b A + c A A) X; out = X.
+ * x: `batch` matrices [rows][cols] of `dtype` at any strides >= 0 (elements), entries of a row neighbours; out: contiguous, may be x if x is.
+ * rows, cols <= 2^20, rows * cols < 2^31.  The coefficients have to keep every singular value in [0, 1] below 8 (the default quintic: 1.21).
+ * ------------------------------------------------------------------------------------------- */
+size_t pwr_orthogonalize_workspace_bytes(int rows, int cols, long long batch);
+int pwr_orthogonalize(const void* x, long long x_batch_stride, long long x_row_stride, void* out, int rows, int cols, long long batch, int dtype,
+                      int steps, float a, float b, float c, float eps, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The optimizer step on flat fp32 buffers that uses it.  A parameter with rows, cols > 1 is a matrix (an OIHW kernel: rows = O, cols = I k k):
+ *   buf = momentum buf + g,  u = nesterov ? g + momentum buf : buf,  p = p (1 - lr weight_decay) - lr update_rms sqrt(max(rows, cols)) orth(u)
+ * (an orthogonal matrix has entries of rms 1 / sqrt(max(rows, cols)): update_rms is the rms of every matrix's update); any other parameter takes
+ * the AdamW step of pwr_adamw_step with buf and v as its moments.  g is multiplied by grad_scale first.  step is 1-based.
+ * The plan of a list is host bytes (pwr_muon_plan writes pwr_muon_plan_bytes of them; 0 / PWR_EINVAL: an empty shape, a negative offset or two
+ * parameters that overlap); plan_dev is a copy of them on the device.  A NULL v is allowed where every parameter is a matrix. */
+typedef struct { long long offset; int rows, cols; } pwr_muon_param;
+size_t pwr_muon_plan_bytes(const pwr_muon_param* params, int n);
+int pwr_muon_plan(const pwr_muon_param* params, int n, void* host_dst);
+size_t pwr_muon_workspace_bytes(const void* plan_host);
+int pwr_muon_step(const void* plan_host, const void* plan_dev, float* p, const float* g, float* buf, float* v, float lr, float momentum, int nesterov,
+                  float weight_decay, float update_rms, int ns_steps, float a, float b, float c, float eps, float beta1, float beta2, float adam_eps,
+                  int step, float grad_scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Input pipeline on the device: /root/reference/datasets.py:243-299 for a batch of raw depth frames

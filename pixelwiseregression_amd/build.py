@@ -30,7 +30,11 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-I" + os.path.
 # the default cap on a pragma-requested unroll (16384 IR instructions, counted BEFORE the per-slot constants fold) stops it silently otherwise
 # (a warning, and a kernel whose register arrays live in scratch)
 # -amdgpu-mfma-vgpr-form: its accumulators live in VGPRs (the epilogue reads them with vector instructions; the AGPR file holds weights)
-PER_FILE_FLAGS = {"conv_wstat.hip": ["-mllvm", "-pragma-unroll-threshold=1000000", "-mllvm", "-amdgpu-mfma-vgpr-form=1", "-Werror=pass-failed"]}
+# likelihood.hip, orth.hip: no packed f32 instructions at all (FLAGS keeps only the vectoriser from making them; the compiler also selects them
+# for float code it finds in pairs)
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+PER_FILE_FLAGS = {"likelihood.hip": NO_PACKED_F32, "orth.hip": NO_PACKED_F32,
+                  "conv_wstat.hip": ["-mllvm", "-pragma-unroll-threshold=1000000", "-mllvm", "-amdgpu-mfma-vgpr-form=1", "-Werror=pass-failed"]}
 # experiment KERNELS that only the debug build compiles and links (never part of the product).  Standalone probes with a main() of their
 # own live in tools/probes/ and are built by their scripts (tools/issue_probe.sh), not into any library.
 DEBUG_SRC = os.path.join(ROOT, "tools", "csrc_debug")

@@ -46,6 +46,8 @@ struct Ctx {
   const float* g_p[8] = {};
   const float* g_D[8] = {};
   const float* g_uvd[8] = {};
+  const float* g_z[8] = {};   // of the heat maps' logits, and of w: for the next backward only (pwr_engine_logit_grad)
+  const float* g_w[8] = {};
   void* stream = nullptr;
   int training = 1;
   // second stream for the parameter-gradient kernels (wgrad + reduce + bias sums): they only feed the flat gradient
@@ -243,6 +245,7 @@ struct Engine {
   size_t bcur = 0;
   // plan
   size_t arena_bytes = 0, pack_bytes = 0;
+  size_t logits_off[8] = {};         // arena offsets of the stages' heat map logits
   std::vector<Op> fwd;
   std::vector<std::vector<Op>> bwd;  // per segment, already in execution order
   std::vector<Op> bwd_cur;           // segment being built (reverse order)
@@ -1309,6 +1312,7 @@ struct Engine {
       R.w_off = method == 0 ? take_param(J) : -1;
       scope = "s" + std::to_string(s) + ".dec";
       R.z = alloc((size_t)B * J * N * 4, "z");
+      logits_off[s] = R.z;
       Head hp, hd;
       heads_fwd(f, R.z, s, hp, hd);
       const size_t zoff = R.z;
@@ -1346,9 +1350,16 @@ struct Engine {
           rc = pwr_decode_bwd(c.out_p[s], (const float*)(c.arena + Rc.z), c.out_D[s], c.label, c.mask, woff >= 0 ? c.params + woff : nullptr,
                               c.out_uvd[s], gH, gD, gU, (float*)(c.arena + Rc.gz), (float*)(c.arena + Rc.gDt),
                               woff >= 0 ? (float*)(c.arena + Rc.gwp) : nullptr, Bc, Jc, Pc, meth, c.stream);
+          if (!rc && c.g_z[s]) rc = pwr_add_inplace(c.g_z[s], c.arena + Rc.gz, n, PWR_F32, c.stream);
+          const float* gw = c.g_w[s];
+          c.g_z[s] = c.g_w[s] = nullptr;
           if (rc || woff < 0) return rc;
           // (the soft-argmax temperature's gradient: a one-block reduce that only feeds the flat gradient -- side stream)
-          return run_on_side(c, [=](Ctx& c2) { return pwr_decode_gw_reduce((const float*)(c2.arena + Rc.gwp), c2.grads + woff, Bc, Jc, 0, c2.stream); });
+          return run_on_side(c, [=](Ctx& c2) {
+            int r = pwr_decode_gw_reduce((const float*)(c2.arena + Rc.gwp), c2.grads + woff, Bc, Jc, 0, c2.stream);
+            if (!r && gw) r = pwr_decode_gw_reduce(gw, c2.grads + woff, 1, Jc, 1, c2.stream);
+            return r;
+          });
         });
         heads_bwd(f, hp, hd, R.gz, R.gDt);
         bwd_cur.insert(bwd_cur.end(), hg_bwd.begin(), hg_bwd.end());
@@ -1534,6 +1545,7 @@ extern "C" int pwr_engine_forward(void* h, const float* img, const float* label,
     c.out_p[s] = (float*)outs[3 * s]; c.out_D[s] = (float*)outs[3 * s + 1]; c.out_uvd[s] = (float*)outs[3 * s + 2];
   }
   e->generation++;
+  for (int k = 0; k < e->stages; ++k) c.g_z[k] = c.g_w[k] = nullptr;
   auto run = [&](void* st) -> int {
     c.stream = st;
     bool pack_wait = false;
@@ -1584,6 +1596,16 @@ extern "C" int pwr_engine_forward(void* h, const float* img, const float* label,
   const int rc = run(stream);
   c.stream = stream;
   return rc;
+}
+extern "C" size_t pwr_engine_logits_offset(void* h, int stage) {
+  Engine* e = (Engine*)h;
+  return stage < 0 || stage >= e->stages ? (size_t)-1 : e->logits_off[stage];
+}
+extern "C" int pwr_engine_logit_grad(void* h, int stage, const float* gz, const float* gw) {
+  Engine* e = (Engine*)h;
+  if (!e->training || stage < 0 || stage >= e->stages || (gw && e->method != 0)) return PWR_EINVAL;
+  e->ctx.g_z[stage] = gz; e->ctx.g_w[stage] = gw;
+  return 0;
 }
 extern "C" long long pwr_engine_generation(void* h) { return ((Engine*)h)->generation; }
 

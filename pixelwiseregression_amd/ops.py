@@ -2,6 +2,8 @@
 
 Only device tensors are accepted: there is no CPU implementation behind these ops by design.
 """
+from typing import NamedTuple, Optional
+
 import torch
 
 from . import _lib
@@ -81,3 +83,223 @@ class DecodeFn(torch.autograd.Function):
 
 def decode(z, D, L, m, w, method="softmax"):
     return DecodeFn.apply(z, D, L, m, w, method)
+
+
+class _on:
+    """Launches go to the tensors' device, whichever is current."""
+
+    def __init__(self, device):
+        self.device = device if device.index not in (None, torch.cuda.current_device()) else None
+
+    def __enter__(self):
+        if self.device is not None:
+            self.before = torch.cuda.current_device()
+            torch.cuda.set_device(self.device)
+
+    def __exit__(self, *a):
+        if self.device is not None:
+            torch.cuda.set_device(self.before)
+
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _dtype_tag(t, what):
+    if t.dtype not in _DTYPES:
+        raise ValueError("%s must be float32 or bfloat16, got %s" % (what, t.dtype))
+    return _DTYPES[t.dtype]
+
+
+def _same_device(t, *others):
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError("tensors on %s and %s" % (t.device, o.device))
+
+
+class LogLikelihood(NamedTuple):
+    """What ``log_likelihood`` returns; ``top_logp`` / ``top_index`` are None without ``topk``."""
+    logp: torch.Tensor
+    entropy: torch.Tensor
+    top_logp: Optional[torch.Tensor]
+    top_index: Optional[torch.Tensor]
+
+
+class _Rows:
+    """The arguments of log_likelihood as the kernels take them: rows of V values, `ld` apart."""
+
+    def __init__(self, z, index, w, mask):
+        if z.dim() not in (2, 3, 4):
+            raise ValueError("z must be [N, V], [B, J, V] or [B, J, H, W], got %s" % (tuple(z.shape),))
+        self.dtype = _dtype_tag(z, "z")
+        self.lead = tuple(z.shape[:1] if z.dim() == 2 else z.shape[:2])
+        self.J = z.shape[1] if z.dim() > 2 else 1
+        v = z.flatten(2) if z.dim() == 4 else z
+        self.rows, self.V = int(torch.Size(self.lead).numel()), v.shape[-1]
+        if self.V < 1:
+            raise ValueError("a row of no values")
+        if self.J < 1:
+            raise ValueError("no joints")
+        if (self.V > 1 and v.stride(-1) != 1) or (v.dim() == 3 and v.shape[0] > 1 and self.J > 1 and v.stride(0) != self.J * v.stride(1)):
+            v = v.contiguous()
+        self.z = v
+        self.ld = v.stride(1) if v.dim() == 3 and self.J > 1 else v.stride(0)
+        if index is not None:
+            if tuple(index.shape) != self.lead or index.is_floating_point() or index.is_complex() or index.dtype == torch.bool:
+                raise ValueError("index must be whole numbers of shape %s, got %s %s" % (self.lead, index.dtype, tuple(index.shape)))
+            index = index.to(torch.int64).contiguous()
+        self.index = index
+        if w is not None:
+            if w.numel() != self.J or not w.is_floating_point():
+                raise ValueError("w must hold one number per joint (%d), got %s" % (self.J, tuple(w.shape)))
+            w = w.detach().reshape(-1).float().contiguous()
+        self.w = w
+        self.mask_rows = 1
+        if mask is not None:
+            m = mask.flatten(2) if z.dim() == 4 and mask.dim() == 4 else mask
+            per_row, per_sample = self.lead + (self.V,), (self.lead[0], 1, self.V)
+            if tuple(m.shape) == per_sample and z.dim() > 2:
+                self.mask_rows = self.J
+            elif tuple(m.shape) != per_row:
+                raise ValueError("mask must be %s or one per sample %s, got %s" % (per_row, per_sample, tuple(mask.shape)))
+            mask = m.detach().float().contiguous()
+        self.mask = mask
+        _same_device(z, index, w, mask)
+
+
+def _likelihood_forward(r, topk, stats):
+    z, dev = r.z, r.z.device
+    logp = torch.empty(r.lead, device=dev, dtype=torch.float32) if r.index is not None else None
+    entropy = torch.empty(r.lead, device=dev, dtype=torch.float32)
+    top_logp = torch.empty(r.lead + (topk,), device=dev, dtype=torch.float32) if topk else None
+    top_index = torch.empty(r.lead + (topk,), device=dev, dtype=torch.int64) if topk else None
+    st = torch.empty(r.rows, 2, device=dev, dtype=torch.float32) if stats else None
+    l = _lib.lib()
+    need = l.pwr_likelihood_workspace_bytes(r.rows, r.V, topk)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    with _on(dev):
+        _lib.check(l.pwr_likelihood_fwd(z.data_ptr(), r.ld, _lib.ptr(r.w), r.J, _lib.ptr(r.mask), r.mask_rows, _lib.ptr(r.index), _lib.ptr(logp),
+                                        _lib.ptr(entropy), _lib.ptr(st), _lib.ptr(top_logp), _lib.ptr(top_index), r.rows, r.V, topk, r.dtype,
+                                        _lib.ptr(ws), need, _lib.stream_ptr(dev)), "pwr_likelihood_fwd")
+    return logp, entropy, top_logp, top_index, st
+
+
+def _likelihood_backward(r, stats, entropy, glogp, gentropy, need_w):
+    dev = r.z.device
+    gz = torch.empty(r.z.shape, device=dev, dtype=r.z.dtype)
+    gw = torch.empty(r.J, device=dev, dtype=torch.float32) if need_w else None
+    glogp, gentropy = (g.contiguous().float() if g is not None else None for g in (glogp, gentropy))
+    l = _lib.lib()
+    need = l.pwr_likelihood_bwd_workspace_bytes(r.rows, r.V) if need_w else 0
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    with _on(dev):
+        _lib.check(l.pwr_likelihood_bwd(r.z.data_ptr(), r.ld, _lib.ptr(r.w), r.J, _lib.ptr(r.mask), r.mask_rows, _lib.ptr(r.index), stats.data_ptr(),
+                                        entropy.data_ptr(), _lib.ptr(glogp), _lib.ptr(gentropy), gz.data_ptr(), _lib.ptr(gw), r.rows, r.V, r.dtype,
+                                        _lib.ptr(ws), need, _lib.stream_ptr(dev)), "pwr_likelihood_bwd")
+    return gz, gw
+
+
+class LogLikelihoodFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, w, index, mask, topk):
+        r = _Rows(z, index, w, mask)
+        logp, entropy, top_logp, top_index, stats = _likelihood_forward(r, topk, True)
+        ctx.save_for_backward(z, w, r.index, r.mask, stats, entropy)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*[t for t in (top_logp, top_index) if t is not None])
+        return logp, entropy, top_logp, top_index
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, glogp, gentropy, _, __):
+        z, w, index, mask, stats, entropy = ctx.saved_tensors
+        if glogp is None and gentropy is None:
+            return (None,) * 5
+        # (mask and index are the kernels' own copies by now: the mask in its row form)
+        r = _Rows(z, index, w, mask)
+        gz, gw = _likelihood_backward(r, stats, entropy, glogp, gentropy, ctx.needs_input_grad[1])
+        return gz.view(z.shape) if ctx.needs_input_grad[0] else None, gw.view(w.shape).to(w.dtype) if gw is not None else None, None, None, None
+
+
+def log_likelihood(z, index, w=None, mask=None, topk=0):
+    """Log likelihood of the pixel ``index`` under every heat map ``softmax(w z)`` -- the distribution ``decode`` reads its joint from
+    (model.py:83-85) --, the map's entropy and its ``topk`` most likely pixels: a loss for the maps, and the confidence and the alternatives of a
+    prediction.
+
+    z: logits ``[B, J, H, W]``, ``[B, J, V]`` or ``[N, V]``, float32 or bfloat16.  index: ``[B, J]`` (``[N]``) whole numbers, -1 where no pixel is
+    given (log likelihood 0, no gradient); a pixel outside its map gives NaN; None: no ``logp``.  w: one number per joint.  mask: ``[B, 1, H, W]``
+    (one per sample) or one per map; 0 = not allowed, whatever z holds there.  topk <= 32: equal values go by the lowest index; what does not exist
+    (masked, -inf, beyond the map) is ``(-inf, -1)``.  A map without an allowed pixel: -inf, entropy 0, zero gradient.
+
+    Returns ``LogLikelihood(logp, entropy, top_logp, top_index)``, float32 (int64 the last); gradients of ``logp`` and ``entropy`` reach z and w."""
+    _require_cuda(z, index, w, mask)
+    topk = int(topk)
+    if not 0 <= topk <= 32:
+        raise ValueError("topk must be 0 .. 32, got %d" % topk)
+    if torch.is_grad_enabled() and (z.requires_grad or (w is not None and w.requires_grad)):
+        return LogLikelihood(*LogLikelihoodFn.apply(z, w, index, mask, topk))
+    return LogLikelihood(*_likelihood_forward(_Rows(z, index, w, mask), topk, False)[:4])
+
+
+def likelihood_gradients(z, index, w, glogp, gentropy, mask=None):
+    """``log_likelihood(z, index, w, mask)`` and, without an autograd graph, the gradients of ``sum(glogp logp) + sum(gentropy entropy)`` with
+    respect to z and w (float32 ``[J]``).  Returns ``(LogLikelihood, gz, gw)``; gw is None without w."""
+    _require_cuda(z, index, w, glogp, gentropy, mask)
+    with torch.no_grad():
+        r = _Rows(z, index, w, mask)
+        for g in (glogp, gentropy):
+            if g is not None and tuple(g.shape) != r.lead:
+                raise ValueError("an upstream gradient must be %s, got %s" % (r.lead, tuple(g.shape)))
+        _same_device(z, glogp, gentropy)
+        logp, entropy, _, _, stats = _likelihood_forward(r, 0, True)
+        gz, gw = _likelihood_backward(r, stats, entropy, glogp, gentropy, w is not None)
+    return LogLikelihood(logp, entropy, None, None), gz.view(z.shape), gw
+
+
+def heatmap_pixels(uvd, P):
+    """The pixel (row-major index of a P x P map) nearest to each normalised joint ``uvd[..., :2]``, -1 where it lies outside: the inverse of the
+    decoder's grid, u = (column - P // 2) / (P - 1) (utils.py:24-35)."""
+    uv = torch.floor(uvd[..., :2].double() * (P - 1) + (P // 2) + 0.5)
+    inside = ((uv >= 0) & (uv <= P - 1)).all(-1)          # (false for NaN)
+    uv = torch.where(inside[..., None], uv, torch.zeros_like(uv)).long()
+    return torch.where(inside, uv[..., 1] * P + uv[..., 0], torch.full_like(uv[..., 0], -1))
+
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
+    """The matrices ``x`` (``[..., rows, cols]``, float32 or bfloat16) made nearly orthogonal by ``steps`` Newton-Schulz products:
+    ``X = x / (|x| + eps)``, then ``X = a X + (b A + c A A) X`` with ``A = X X^T`` (of the shorter side).  With the default coefficients every singular
+    value above about 1e-3 of the norm ends up between 0.7 and 1.2.  Float32: the precision of float32 products; bfloat16: 2e-3 of the result.
+
+    Not differentiable (it is what an optimizer does to a gradient): a tensor that requires a gradient is refused."""
+    _require_cuda(x, out)
+    tag = _dtype_tag(x, "x")
+    if x.dim() < 2:
+        raise ValueError("x must be a matrix or a batch of them, got %s" % (tuple(x.shape),))
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise NotImplementedError("orthogonalize has no gradient: detach x")
+    a, b, c = (float(t) for t in coefficients)
+    steps = int(steps)
+    if not 1 <= steps <= 64 or not float(eps) >= 0.0:
+        raise ValueError("steps must be 1 .. 64 and eps not negative, got %d, %g" % (steps, eps))
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
+        raise ValueError("out must be a contiguous %s tensor of shape %s" % (x.dtype, tuple(x.shape)))
+    _same_device(x, out)
+    if x.numel() == 0:
+        return out
+    rows, cols = x.shape[-2:]
+    v = x if x.dim() == 3 else x.reshape(-1, rows, cols)
+    if (cols > 1 and v.stride(2) != 1) or (v is not x and v.data_ptr() != x.data_ptr()):
+        v = v.contiguous()
+    l = _lib.lib()
+    need = l.pwr_orthogonalize_workspace_bytes(rows, cols, v.shape[0])
+    if need == 0:
+        raise ValueError("matrices of %d x %d are larger than orthogonalize takes (2^20 a side, 2^31 entries)" % (rows, cols))
+    ws = torch.empty(need, device=x.device, dtype=torch.uint8)
+    with _on(x.device):
+        _lib.check(l.pwr_orthogonalize(v.data_ptr(), v.stride(0), v.stride(1), out.data_ptr(), rows, cols, v.shape[0], tag, steps, a, b, c, float(eps),
+                                       ws.data_ptr(), need, _lib.stream_ptr(x.device)), "pwr_orthogonalize")
+    return out

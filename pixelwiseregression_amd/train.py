@@ -7,7 +7,11 @@
 Forward = one engine call, loss + output gradients = `pwr_loss_sqdiff` (train.py:195-205; with alpha == 1 the dense
 heat-map / depth-map terms have weight zero and are skipped instead of being multiplied by 0), backward = one engine call per
 segment (with the RCCL all-reduce of ddp.DataParallel in between), update = `pwr_adamw_step` / `pwr_sgd_step` on the flat
-parameter buffer (torch.optim.AdamW(weight_decay=0) / SGD(momentum=beta1) semantics, train.py:139-142).
+parameter buffer (torch.optim.AdamW(weight_decay=0) / SGD(momentum=beta1) semantics, train.py:139-142), or `optim.Muon` (opt='muon').
+
+Beside the reference's three terms: lambda_nll > 0 adds lambda_nll * mean_{b,j} -log p(the joint's pixel) per stage, p the heat map as a distribution
+over pixels (`ops.log_likelihood` on the engine's logits), lambda_entropy lambda_entropy * mean entropy.  A joint outside the map has no pixel and adds
+no likelihood.
 """
 import ctypes
 
@@ -15,13 +19,19 @@ import torch
 
 from . import _lib
 from .engine import _get_plan, _run_forward, BF16, F32
+from .ops import heatmap_pixels, likelihood_gradients
+from .optim import Muon
 
 
 class TrainStep:
     def __init__(self, model, opt="adam", lr=1e-3, beta1=0.9, beta2=0.999, weight_decay=0.0, eps=1e-8, alpha=1.0, lambda_h=1.0,
-                 lambda_d=0.01, decay_epoch=15, lr_decay=0.2, target_kernel_size=7, target_sigmoid=1.5):
-        if opt not in ("adam", "sgd"):
-            raise ValueError("opt must be 'adam' or 'sgd' (train.py:139-142)")
+                 lambda_d=0.01, decay_epoch=15, lr_decay=0.2, target_kernel_size=7, target_sigmoid=1.5, momentum=0.95, lambda_nll=0.0,
+                 lambda_entropy=0.0):
+        if opt not in ("adam", "sgd", "muon"):
+            raise ValueError("opt must be 'adam' or 'sgd' (train.py:139-142) or 'muon'")
+        self.lambda_nll, self.lambda_entropy = float(lambda_nll), float(lambda_entropy)
+        if (self.lambda_nll or self.lambda_entropy) and model.heatmap_method != "softmax":
+            raise ValueError("lambda_nll / lambda_entropy need heat maps that are a softmax of logits (heatmap_method='softmax')")
         self.model, self.opt = model, opt
         self.lr, self.beta1, self.beta2, self.wd, self.eps = lr, beta1, beta2, weight_decay, eps
         self.alpha, self.lambda_h, self.lambda_d = alpha, lambda_h, lambda_d
@@ -30,7 +40,9 @@ class TrainStep:
         self.steps, self.epochs = 0, 0
         flat = model.flat_parameters()
         self.m = torch.zeros_like(flat)
-        self.v = torch.zeros_like(flat) if opt == "adam" else None
+        self.v = torch.zeros_like(flat) if opt != "sgd" else None
+        self.muon = Muon.for_model(model, momentum=momentum, weight_decay=weight_decay, beta1=beta1, beta2=beta2, adam_eps=eps, buf=self.m,
+                                   v=self.v) if opt == "muon" else None
         self.loss = torch.zeros(1, device=flat.device)
         self._scratch = None
 
@@ -96,6 +108,7 @@ class TrainStep:
                                          self.loss.data_ptr(), 0 if first else 1, n_uvd, stream), "pwr_loss_sqdiff")
             first = False
             ptrs += [gh.data_ptr() if gh is not None else None, gd.data_ptr() if gd is not None else None, gu.data_ptr()]
+        likelihood = self._likelihood(plan, uvd) if self.lambda_nll or self.lambda_entropy else None
         arr = (ctypes.c_void_p * len(ptrs))(*ptrs)
         grad = m.flat_grad()
         plan.bind(m, grad)
@@ -113,8 +126,29 @@ class TrainStep:
         if self.opt == "adam":
             _lib.check(l.pwr_adamw_step(flat.data_ptr(), grad.data_ptr(), self.m.data_ptr(), self.v.data_ptr(), n, self.lr, self.beta1,
                                         self.beta2, self.eps, self.wd, self.steps, scale, stream), "pwr_adamw_step")
+        elif self.opt == "muon":
+            self.muon.flat, self.muon.lr, self.muon.weight_decay, self.muon.steps = flat, self.lr, self.wd, self.steps - 1
+            self.muon.step(grad, scale)
         else:
             _lib.check(l.pwr_sgd_step(flat.data_ptr(), grad.data_ptr(), self.m.data_ptr(), n, self.lr, self.beta1, self.wd,
                                       1 if self.steps == 1 else 0, scale, stream), "pwr_sgd_step")
-        self._keep = (outs, img, label_img, mask, uvd)      # alive until the next step: the stream may still read them
+        self._keep = (outs, img, label_img, mask, uvd, likelihood)      # alive until the next step: the stream may still read them
         return self.loss.clone()      # a fresh tensor per step (self.loss is overwritten by the next step)
+
+    def _likelihood(self, plan, uvd):
+        """The likelihood terms of every stage: added to the loss, their gradients handed to the engine's next backward.  Returns what has to live
+        until it has run."""
+        m, l = self.model, _lib.lib()
+        B, J, P = plan.B, m.joints, m.label_size
+        index = heatmap_pixels(uvd, P)
+        gl = torch.full((B, J), -self.lambda_nll / (B * J), device=uvd.device)
+        ge = torch.full((B, J), self.lambda_entropy / (B * J), device=uvd.device)
+        keep = [index, gl, ge]
+        for s in range(m.stage):
+            off = l.pwr_engine_logits_offset(plan.h, s)
+            z = plan.arena[off:off + B * J * P * P * 4].view(torch.float32).view(B, J, P, P)
+            r, gz, gw = likelihood_gradients(z, index, m.stages[s].plane_regression.w, gl, ge)
+            self.loss += (gl * r.logp + ge * r.entropy).sum()
+            _lib.check(l.pwr_engine_logit_grad(plan.h, s, gz.data_ptr(), gw.data_ptr()), "pwr_engine_logit_grad")
+            keep += [z, r, gz, gw]
+        return keep
