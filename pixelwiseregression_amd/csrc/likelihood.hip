@@ -21,7 +21,10 @@ namespace pwr {
 
 constexpr int kLikeMaxTop = 32;         // of the K most likely pixels
 constexpr int kLikeCand = 256;          // candidates the selection sorts (one per thread)
-constexpr int kLikeChunk = 16384;       // values of a row one workgroup holds in registers (256 threads x 64)
+constexpr int kLikeChunk = 16384;       // values of a row one workgroup holds in registers (512 threads x 32)
+// Without alternatives a workgroup walks a row of over 4096 values; only a row of several chunks is split over workgroups, where there are fewer
+// rows than this.  Walked / split: 512 rows of 50001 fp32 18.6 / 24.0 us, bf16 19.6 / 22.2; 256 rows 13.0 / 15.4 and 15.3 / 13.9.
+constexpr int kLikeWalkRows = 512;
 constexpr int kLikeWaveMax = 512;       // rows up to here: one wave per row (64 lanes x 8)
 
 struct LikeArgs {
@@ -38,118 +41,175 @@ struct LikeArgs {
   float* cand_s; int* cand_i;           // [rows][chunks][K]
 };
 
-// four neighbouring values of T at any element alignment (rows of odd length start anywhere; the hardware takes such an address)
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Quad { T v[4]; };
+// 16 bytes of T at any element alignment (rows of odd length start anywhere; the hardware takes such an address)
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[16 / sizeof(T)]; };
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, int i, int V, float (&o)[4], float fill) {
-  if (i + 3 < V) {
-    const Quad<T> q = *reinterpret_cast<const Quad<T>*>(p + i);
+// VPT of a row's n values per thread, 16 bytes at a time, and the mask's: value k belongs to index value_index(k).  No load hides behind a branch (one
+// that does is waited for before the next is sent): where the workgroup has room for more than n values, every piece is read at an index that has one,
+// n >= N (or N values in front of p), and moved into place by values().
+template <typename T, int NT, int VPT>
+struct RowPart {
+  static constexpr int N = 16 / sizeof(T);
+  Piece<T> q[VPT / N];
+  Piece<float> mq[VPT / 4];
+  __device__ __forceinline__ void load(const T* p, const float* mask, int n) {
+    const int tid = threadIdx.x;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = Elem<T>::to_f(q.v[k]);
-  } else {
+    for (int k = 0; k < VPT / N; ++k) q[k] = *reinterpret_cast<const Piece<T>*>(p + min((k * NT + tid) * N, n - N));
+    if (mask) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = i + k < V ? Elem<T>::to_f(p[i + k]) : fill;
+      for (int k = 0; k < VPT / 4; ++k)
+        mq[k] = *reinterpret_cast<const Piece<float>*>(mask + min((k * 4 / N * NT + tid) * N, n - N) + k * 4 % N);
+    }
   }
+  // v = z, s = w z of the allowed ones, -inf where the mask says so and beyond n
+  __device__ __forceinline__ void values(bool mask, int n, float w, float (&v)[VPT], float (&s)[VPT]) const {
+    const int tid = threadIdx.x;
+    if (n >= NT * VPT) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) { v[k] = Elem<T>::to_f(q[k / N].v[k % N]); s[k] = v[k] * w; }
+      if (mask) {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) s[k] = mq[k / 4].v[k % 4] == 0.f ? -INFINITY : s[k];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VPT / N; ++k) {
+        const int d = (k * NT + tid) * N - (n - N);             // how far the piece reaches beyond n
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          float x = Elem<T>::to_f(q[k].v[e]), in = mask ? mq[(k * N + e) / 4].v[e % 4] : 1.f;
+#pragma unroll
+          for (int j = e + 1; j < N; ++j) {
+            x = d == j - e ? Elem<T>::to_f(q[k].v[j]) : x;
+            in = mask && d == j - e ? mq[(k * N + j) / 4].v[j % 4] : in;
+          }
+          v[k * N + e] = x;
+          s[k * N + e] = e + d < N && in != 0.f ? x * w : -INFINITY;
+        }
+      }
+    }
+  }
+};
+// the index of value k of a RowPart
+template <typename T, int NT>
+__device__ __forceinline__ int value_index(int k) {
+  constexpr int N = 16 / sizeof(T);
+  return ((k / N) * NT + (int)threadIdx.x) * N + k % N;
 }
 
-// The statistics of a set of values, and how two sets join.  M = -inf: nothing in the set (c = q = 0, r = 0 or NaN).
+// The statistics of a set of values, and how sets join.  M = -inf: nothing in the set (c = q = 0, r = 0 or NaN).
 struct LikeStat { float M, c, r, q; };
-__device__ __forceinline__ LikeStat like_join(const LikeStat& a, const LikeStat& b) {
-  const float M = fmaxf(a.M, b.M);
-  LikeStat o = {M, 0.f, 0.f, 0.f};
-  auto add = [&](const LikeStat& x) {
-    if (x.M == M) { o.c += x.c; o.r += x.r; o.q += x.q; }
-    else if (x.M == -INFINITY) { o.r += x.r; }                     // (empty: adds 0, or the NaN it saw)
-    else {
-      const float d = x.M - M, f = __expf(d), t = x.c + x.r;
-      o.r += f * t;
-      if (f > 0.f) o.q += f * (x.q + d * t);
-    }
-  };
-  add(a); add(b);
-  return o;
+// x's sums relative to the joint maximum M >= x.M
+__device__ __forceinline__ LikeStat like_shift(const LikeStat& x, float M) {
+  if (x.M == M) return x;
+  if (x.M == -INFINITY) return {M, 0.f, x.r, 0.f};                  // (empty: adds 0, or the NaN it saw)
+  const float d = x.M - M, f = __expf(d), t = x.c + x.r;
+  return {M, 0.f, f * t, f > 0.f ? f * (x.q + d * t) : 0.f};
 }
 // log of the sum of exp(s - M)
 __device__ __forceinline__ float like_log_total(const LikeStat& a) {
-  if (a.c == 0.f && a.r == 0.f) return -INFINITY;
-  return a.c > 0.f ? (a.c == 1.f ? 0.f : logf(a.c)) + log1pf(a.r / a.c) : a.r * INFINITY;      // (c == 0 with r != 0: a NaN was seen)
+  if (a.c == 0.f) return a.r == 0.f ? -INFINITY : a.r * INFINITY;                // (nothing, or a NaN was seen)
+  return a.c == 1.f ? log1pf(a.r) : __logf(a.c + a.r);                            // (from 2 on the sum swallows nothing)
 }
 
+// The given pixel t of a row: its s, or NaN for one that is no pixel.  Its index is read at the start of a kernel and s behind the row's own loads, so
+// that the two reads in a row cost no time of their own.
+struct LikeGiven { bool any; float s; };
 template <typename T>
-__device__ __forceinline__ float like_value(const LikeArgs& a, long long row, long long t, float w) {
-  const float s = Elem<T>::to_f(reinterpret_cast<const T*>(a.z)[row * a.ldz + t]) * w;
-  return a.mask && a.mask[(row / a.mask_rows) * a.V + t] == 0.f ? -INFINITY : s;
+__device__ __forceinline__ LikeGiven like_given(const LikeArgs& a, long long t, const T* z, const float* mask, float w) {
+  if (t < 0) return {false, 0.f};
+  if (t >= a.V) return {true, NAN};                                // (nothing is read, and the result is loud)
+  const float s = Elem<T>::to_f(z[t]) * w;
+  return {true, mask && mask[t] == 0.f ? -INFINITY : s};
 }
 
 // what one thread writes for a finished row
-template <typename T>
-__device__ __forceinline__ float like_finish(const LikeArgs& a, long long row, const LikeStat& st, float w) {
-  const float lt = like_log_total(st);
+__device__ __forceinline__ void like_finish(const LikeArgs& a, unsigned row, const LikeStat& st, float lt, const LikeGiven& g) {
   const bool none = st.c == 0.f && st.r == 0.f;
   if (a.logp) {
     float lp = 0.f;
-    const long long t = a.index ? a.index[row] : -1;
-    if (t >= a.V) lp = NAN;                                        // (not a pixel: loud, and nothing is read)
-    else if (t >= 0) {
-      const float s = like_value<T>(a, row, t, w);
-      lp = none || s == -INFINITY ? (lt == lt ? -INFINITY : lt) : (s - st.M) - lt;
-    }
+    if (g.any) lp = g.s != g.s ? NAN : none || g.s == -INFINITY ? (lt == lt ? -INFINITY : lt) : (g.s - st.M) - lt;
     a.logp[row] = lp;
   }
   if (a.entropy) a.entropy[row] = none ? 0.f : lt - st.q / (st.c + st.r);
-  if (a.stats) { a.stats[2 * row] = st.M; a.stats[2 * row + 1] = lt; }
-  return lt;
+  if (a.stats) { a.stats[2ll * row] = st.M; a.stats[2ll * row + 1] = lt; }
 }
 
 // (s, i) before (t, j) in the order of the alternatives: the larger value, among equals the lower index
 __device__ __forceinline__ bool like_before(float s, int i, float t, int j) { return s > t || (s == t && i < j); }
 
-// The K first of the (s, i) a workgroup of 256 threads holds, in order, to emit(rank, s, i); ranks beyond what is there get (-inf, -1).
-// The K-th largest of the threads' own maxima bounds the K-th value from below (K threads hold one each): what reaches it are the candidates,
-// rarely more than a few over K, sorted by counting who comes before whom.  More candidates than threads (long ties): K rounds of a
-// maximum over what comes after the last one instead.
-template <int VPT, typename IndexOf, typename Emit>
-__device__ __forceinline__ void like_select(const float (&s)[VPT], IndexOf index_of, int K, char* lds, Emit emit) {
-  float* tm = reinterpret_cast<float*>(lds);                       // [256] maxima, then candidates' values
-  int* ti = reinterpret_cast<int*>(lds + 1024);                    // [256] candidates' indices
-  int* cnt = reinterpret_cast<int*>(lds + 2048);
-  float* thr = reinterpret_cast<float*>(lds + 2052);
-  const int tid = threadIdx.x;
-  float m = -INFINITY;
+// Shared memory of a workgroup of NW waves.
+template <int NW> struct LikeShared {
+  float group[NW][32];
+  float sum[3][NW];
+  int count;
+  __attribute__((aligned(16))) float cs[kLikeCand];
+  __attribute__((aligned(16))) int ci[kLikeCand];
+};
+
+// The workgroup's maximum, and a bound that at least K of its values reach: the values fall into G >= K groups (lane mod G, over all waves), each group's
+// maximum is a value, so K values reach the least of these maxima -- and by the coupon collector's count about G ln G values do in all.
+// One barrier.  m: this thread's maximum.
+template <int NW>
+__device__ __forceinline__ void like_maximum(float m, int K, LikeShared<NW>& sh, float& M, float& bound) {
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  m = fmaxf(m, lane_xor<32>(m));
+  if (lane < 32) sh.group[wid][lane] = m;
+  if (threadIdx.x == 0) sh.count = 0;
+  if (K)
+    for (int k = threadIdx.x; k < kLikeCand; k += NW * 64) sh.cs[k] = -INFINITY;
+  __syncthreads();
+  m = sh.group[0][lane & 31];
 #pragma unroll
-  for (int k = 0; k < VPT; ++k) m = fmaxf(m, s[k]);
-  __syncthreads();
-  tm[tid] = m;
-  if (tid == 0) *cnt = 0;
-  __syncthreads();
-  int rank = 0;
-  for (int k = 0; k < 256; k += 4) {
-    const f32x4 o = *reinterpret_cast<const f32x4*>(tm + k);
+  for (int w = 1; w < NW; ++w) m = fmaxf(m, sh.group[w][lane & 31]);
+  if (K <= 16) m = fmaxf(m, lane_xor<16>(m));
+  if (K <= 8) m = fmaxf(m, lane_xor<8>(m));
+  if (K <= 4) m = fmaxf(m, lane_xor<4>(m));
+  float lo = m, hi = m;
+  lo = fminf(lo, lane_xor<16>(lo)); hi = fmaxf(hi, lane_xor<16>(hi));
+  lo = fminf(lo, lane_xor<8>(lo)); hi = fmaxf(hi, lane_xor<8>(hi));
+  lo = fminf(lo, lane_xor<4>(lo)); hi = fmaxf(hi, lane_xor<4>(hi));
+  lo = fminf(lo, lane_xor<2>(lo)); hi = fmaxf(hi, lane_xor<2>(hi));
+  lo = fminf(lo, lane_xor<1>(lo)); hi = fmaxf(hi, lane_xor<1>(hi));
+  M = hi; bound = lo;
+}
+
+// What reaches the bound becomes a candidate (in any order); a barrier has to follow.  own: this thread's maximum.
+template <int NW, int VPT, typename IndexOf>
+__device__ __forceinline__ void like_push(LikeShared<NW>& sh, const float (&s)[VPT], IndexOf index_of, float own, float bound) {
+  if (own < bound || own == -INFINITY) return;
+  int n = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) rank += o[e] > m || (o[e] == m && k + e < tid);
-  }
-  if (rank == K - 1) *thr = m;
-  __syncthreads();
-  const float bound = *thr;
-  if (m >= bound && m > -INFINITY) {
+  for (int k = 0; k < VPT; ++k) n += s[k] >= bound && s[k] > -INFINITY;
+  int at = atomicAdd(&sh.count, n);
 #pragma unroll
-    for (int k = 0; k < VPT; ++k)
-      if (s[k] >= bound && s[k] > -INFINITY) {
-        const int at = atomicAdd(cnt, 1);                          // (the order of arrival is not the order of the result)
-        if (at < kLikeCand) { tm[at] = s[k]; ti[at] = index_of(k); }
-      }
-  }
-  __syncthreads();
-  const int n = *cnt;
+  for (int k = 0; k < VPT; ++k)
+    if (s[k] >= bound && s[k] > -INFINITY) {
+      if (at < kLikeCand) { sh.cs[at] = s[k]; sh.ci[at] = index_of(k); }
+      ++at;
+    }
+}
+
+// The K first of the workgroup's (s, i) in order, to emit(rank, s, i); ranks beyond what is there get (-inf, -1).  Candidates are placed by counting
+// who comes before them; more of them than there is room for (long ties, or a mask that leaves one group empty): K rounds of a maximum over what
+// comes after the last one.
+template <int NW, int VPT, typename IndexOf, typename Emit>
+__device__ __forceinline__ void like_select(const float (&s)[VPT], IndexOf index_of, int K, LikeShared<NW>& sh, Emit emit) {
+  const int tid = threadIdx.x, n = sh.count;
   if (n <= kLikeCand) {
-    if (tid < n) {
-      const float v = tm[tid];
-      const int i = ti[tid];
+    for (int c = tid; c < n; c += NW * 64) {
+      const float v = sh.cs[c];
+      const int i = sh.ci[c];
       int r = 0;
-      for (int k = 0; k < n; ++k) r += like_before(tm[k], ti[k], v, i);
+      for (int k = 0; k < n; k += 4) {                               // (beyond n: -inf, which comes before nobody)
+        const f32x4 x = *reinterpret_cast<const f32x4*>(sh.cs + k);
+        const int4 j = *reinterpret_cast<const int4*>(sh.ci + k);
+        r += like_before(x.x, j.x, v, i) + like_before(x.y, j.y, v, i) + like_before(x.z, j.z, v, i) + like_before(x.w, j.w, v, i);
+      }
       if (r < K) emit(r, v, i);
-    } else if (tid < K) emit(tid, -INFINITY, -1);                  // (n < K only when that is all there is)
+    }
+    for (int r = n + tid; r < K; r += NW * 64) emit(r, -INFINITY, -1);       // (n < K only when that is all there is)
     return;
   }
   float last_s = INFINITY;
@@ -168,140 +228,233 @@ __device__ __forceinline__ void like_select(const float (&s)[VPT], IndexOf index
       if (like_before(xs, xi, bs, bi)) { bs = xs; bi = xi; }
     }
     __syncthreads();
-    if ((tid & 63) == 0) { tm[tid >> 6] = bs; ti[tid >> 6] = bi; }
+    if ((tid & 63) == 0) { sh.cs[tid >> 6] = bs; sh.ci[tid >> 6] = bi; }
     __syncthreads();
-    bs = tm[0]; bi = ti[0];
+    bs = sh.cs[0]; bi = sh.ci[0];
 #pragma unroll
-    for (int k = 1; k < 4; ++k)
-      if (like_before(tm[k], ti[k], bs, bi)) { bs = tm[k]; bi = ti[k]; }
+    for (int k = 1; k < NW; ++k)
+      if (like_before(sh.cs[k], sh.ci[k], bs, bi)) { bs = sh.cs[k]; bi = sh.ci[k]; }
     if (tid == 0) emit(r, bs, bs > -INFINITY ? bi : -1);
     last_s = bs; last_i = bi;
   }
 }
 
-// One workgroup: one chunk of one row (CHUNKED), or a whole row.
-template <typename T, int VPT, bool CHUNKED>
-__global__ __launch_bounds__(256) void like_fwd_kernel(LikeArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[2064];
-  __shared__ float red[16];
-  const int tid = threadIdx.x;
-  const long long row = CHUNKED ? (long long)blockIdx.x / a.chunks : blockIdx.x;
-  const int ch = CHUNKED ? (int)(blockIdx.x - row * a.chunks) : 0;
-  const int base = ch * a.chunk, end = CHUNKED ? min(a.V, base + a.chunk) : a.V;
-  const float w = a.w ? a.w[row % a.J] : 1.f;
+// One workgroup: one chunk of one row (CHUNKED), or a whole row.  Two barriers: maximum and bound, then sums and candidates.
+template <typename T, int NT, int VPT, bool CHUNKED, bool TOP>
+__device__ __forceinline__ void like_fwd_block(const LikeArgs& a, LikeShared<NT / 64>& sh, unsigned row, int base, int n) {
+  constexpr int NW = NT / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const float w = a.w ? a.w[row % (unsigned)a.J] : 1.f;
   const T* z = reinterpret_cast<const T*>(a.z) + row * a.ldz;
-  const float* mk = a.mask ? a.mask + (row / a.mask_rows) * a.V : nullptr;
-  float s[VPT];
+  const float* mrow = a.mask ? a.mask + (long long)(row / (unsigned)a.mask_rows) * a.V : nullptr;
+  const long long t = !CHUNKED && a.index ? a.index[row] : -1;
+  RowPart<T, NT, VPT> part;
+  part.load(z + base, mrow ? mrow + base : nullptr, n);
+  const LikeGiven given = like_given<T>(a, t, z, mrow, w);
+  float s[VPT], v[VPT];
+  part.values(mrow != nullptr, n, w, v, s);
+  float own = -INFINITY, m, bound;
 #pragma unroll
-  for (int k = 0; k < VPT / 4; ++k) {
-    const int i = base + (k * 256 + tid) * 4;
-    float v[4];
-    load4(z, i, end, v, 0.f);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[4 * k + e] = i + e < end ? v[e] * w : -INFINITY;
-  }
-  if (mk) {
-#pragma unroll
-    for (int k = 0; k < VPT / 4; ++k) {
-      const int i = base + (k * 256 + tid) * 4;
-      float v[4];
-      load4(mk, i, end, v, 0.f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (v[e] == 0.f) s[4 * k + e] = -INFINITY;
-    }
-  }
-  float m = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < VPT; ++k) m = fmaxf(m, s[k]);
-  m = block_max<4>(m, red);
+  for (int k = 0; k < VPT; ++k) own = fmaxf(own, s[k]);
+  like_maximum<NW>(own, a.K, sh, m, bound);
   const float m0 = m == -INFINITY ? 0.f : m;
-  float sum[3] = {0.f, 0.f, 0.f};
+  float c = 0.f, r = 0.f, q = 0.f;
+  if (__any(own == m0)) {
+    // the wave that has the maximum (or a few): its values at the maximum are counted, the others summed
 #pragma unroll
-  for (int k = 0; k < VPT; ++k) {
-    const float d = s[k] - m0, e = __expf(d);
-    const bool at = d == 0.f && m0 == m;
-    sum[0] += at ? 1.f : 0.f;
-    sum[1] += at ? 0.f : e;
-    if (e != 0.f) sum[2] = fmaf(e, d, sum[2]);                     // (0 x -inf is 0 here; NaN passes)
-  }
-  block_sum<3, 4>(sum, red);
-  const LikeStat st = {m, sum[0], sum[1], sum[2]};
-  auto index_of = [&](int k) { return base + ((k >> 2) * 256 + tid) * 4 + (k & 3); };
-  if constexpr (CHUNKED) {
-    if (tid == 0) *reinterpret_cast<f32x4*>(a.part + 4 * (long long)blockIdx.x) = f32x4{st.M, st.c, st.r, st.q};
-    if (a.K) {
-      float* cs = a.cand_s + (long long)blockIdx.x * a.K;
-      int* ci = a.cand_i + (long long)blockIdx.x * a.K;
-      like_select<VPT>(s, index_of, a.K, lds, [&](int r, float v, int i) { cs[r] = v; ci[r] = i; });
+    for (int k = 0; k < VPT; ++k) {
+      const float d = s[k] - m0, e = __expf(d);
+      const bool at = d == 0.f && m0 == m;
+      c += at ? 1.f : 0.f;
+      r += at ? 0.f : e;
+      q = fmaf(e, fmaxf(d, -1e30f), q);
     }
   } else {
-    if (tid == 0) like_finish<T>(a, row, st, w);
-    if (a.K) {
-      const float lt = like_log_total(st);
-      float* ts = a.top_logp + row * a.K;
-      long long* ix = a.top_index + row * a.K;
-      like_select<VPT>(s, index_of, a.K, lds, [&](int r, float v, int i) { ts[r] = i < 0 ? v : (v - st.M) - lt; ix[r] = i; });
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const float d = s[k] - m0, e = __expf(d);
+      r += e;
+      q = fmaf(e, fmaxf(d, -1e30f), q);                            // (0 x -inf is 0 here; a NaN has passed through e)
+    }
+  }
+  c = wave_sum(c); r = wave_sum(r); q = wave_sum(q);
+  if (lane == 0) { sh.sum[0][wid] = c; sh.sum[1][wid] = r; sh.sum[2][wid] = q; }
+  auto index_of = [&](int k) { return base + value_index<T, NT>(k); };
+  if constexpr (TOP) like_push<NW, VPT>(sh, s, index_of, own, bound);
+  __syncthreads();
+  c = r = q = 0.f;
+#pragma unroll
+  for (int k = 0; k < NW; ++k) { c += sh.sum[0][k]; r += sh.sum[1][k]; q += sh.sum[2][k]; }
+  const LikeStat st = {m, c, r, q};
+  if constexpr (CHUNKED) {
+    if (tid == 0) *reinterpret_cast<f32x4*>(a.part + 4 * (long long)blockIdx.x) = f32x4{st.M, st.c, st.r, st.q};
+    if constexpr (TOP) {
+      float* cs = a.cand_s + (long long)blockIdx.x * a.K;
+      int* ci = a.cand_i + (long long)blockIdx.x * a.K;
+      like_select<NW, VPT>(s, index_of, a.K, sh, [&](int rk, float v, int i) { cs[rk] = v; ci[rk] = i; });
+    }
+  } else {
+    const float lt = like_log_total(st);
+    if (tid == NT - 1) like_finish(a, row, st, lt, given);         // (not a thread that has an alternative to place)
+    if constexpr (TOP) {
+      float* ts = a.top_logp + (long long)row * a.K;
+      long long* ix = a.top_index + (long long)row * a.K;
+      like_select<NW, VPT>(s, index_of, a.K, sh, [&](int rk, float v, int i) { ts[rk] = i < 0 ? v : (v - st.M) - lt; ix[rk] = i; });
     }
   }
 }
 
-// Joins the chunks of a row: one workgroup per row, the candidates of all chunks (at most 256 x VPT) selected again.
+// (Straight-line code runs once per workgroup and the instruction cache starts cold: rows of up to 4096 values take one 16-byte piece a thread, long ones 32
+// values.  128 x 42 maps of 128 x 128, fp32: 512 threads x 32 values 74 us = 4.8 TB/s, 1024 x 16 82 us, 256 x 64 79 us.  Alternatives are a form of
+// their own: compiled in and unused they took 50 us of the same launch, in registers and copies.)
+template <typename T, int NT, int VPT, bool CHUNKED, bool TOP>
+__global__ __launch_bounds__(NT) void like_fwd_kernel(LikeArgs a) {
+  __shared__ LikeShared<NT / 64> sh;
+  constexpr int N = 16 / sizeof(T);
+  if constexpr (CHUNKED) {
+    const unsigned row = blockIdx.x / (unsigned)a.chunks;          // (below 2^31: 64-bit divisions would cost more than the loads)
+    const int base = (int)(blockIdx.x - row * (unsigned)a.chunks) * a.chunk, n = min(a.V - base, a.chunk);
+    if (VPT > N && n <= NT * N) like_fwd_block<T, NT, N, true, TOP>(a, sh, row, base, n);       // (a row's short end)
+    else like_fwd_block<T, NT, VPT, true, TOP>(a, sh, row, base, n);
+  } else like_fwd_block<T, NT, VPT, false, TOP>(a, sh, blockIdx.x, 0, a.V);
+}
+
+// Long rows, enough of them to fill the chip, without alternatives: one workgroup walks its row in parts of NT x VPT values, the next part's loads under
+// way while it works on one.  The sums are kept relative to the largest value so far, per thread; one barrier per part.  4096 rows of 50001 bf16: 256 threads
+// x 16 values 102 us = 4.0 TB/s (50000, rows that start aligned: 88 us = 4.7), 256 x 32 112, 512 x 16 128, 1024 x 16 189, a workgroup per chunk and a
+// join 161; 5376 rows of 16384 fp32: 64 us = 5.5 TB/s against 74 in one piece.
+template <typename T, int NT, int VPT>
+__global__ __launch_bounds__(NT) void like_walk_kernel(LikeArgs a) {
+  constexpr int NW = NT / 64, N = 16 / sizeof(T), PART = NT * VPT;
+  __shared__ float top[2][NW], sum[3][NW];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const unsigned row = blockIdx.x;
+  const float w = a.w ? a.w[row % (unsigned)a.J] : 1.f;
+  const T* z = reinterpret_cast<const T*>(a.z) + row * a.ldz;
+  const float* mrow = a.mask ? a.mask + (long long)(row / (unsigned)a.mask_rows) * a.V : nullptr;
+  const long long t = a.index ? a.index[row] : -1;
+  RowPart<T, NT, VPT> part;
+  part.load(z, mrow, a.V);
+  const LikeGiven given = like_given<T>(a, t, z, mrow, w);
+  float M = -INFINITY, c = 0.f, r = 0.f, q = 0.f;
+  for (int base = 0, turn = 0; base < a.V; base += PART, turn ^= 1) {
+    const int n = a.V - base;
+    float s[VPT], v[VPT];
+    part.values(mrow != nullptr, n, w, v, s);
+    if (base + PART < a.V) part.load(z + base + PART, mrow ? mrow + base + PART : nullptr, n - PART);
+    float own = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) own = fmaxf(own, s[k]);
+    const float mw = wave_max(own);
+    if (lane == 0) top[turn][wid] = mw;
+    __syncthreads();                                               // (the other buffer is read by nobody any more)
+    float m = M;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) m = fmaxf(m, top[turn][k]);
+    if (m > M) {
+      const LikeStat x = like_shift(LikeStat{M, c, r, q}, m);
+      c = x.c; r = x.r; q = x.q; M = m;
+    }
+    const float m0 = M == -INFINITY ? 0.f : M;
+    if (__any(own == m0 && M > -INFINITY)) {                        // a wave that has values at the maximum counts them
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        const float d = s[k] - m0, x = __expf(d);
+        const bool at = d == 0.f;
+        c += at ? 1.f : 0.f;
+        r += at ? 0.f : x;
+        q = fmaf(x, fmaxf(d, -1e30f), q);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VPT / N; ++k) {
+        if (k * NT * N >= n) continue;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float d = s[k * N + e] - m0, x = __expf(d);
+          r += x;
+          q = fmaf(x, fmaxf(d, -1e30f), q);
+        }
+      }
+    }
+  }
+  c = wave_sum(c); r = wave_sum(r); q = wave_sum(q);
+  if (lane == 0) { sum[0][wid] = c; sum[1][wid] = r; sum[2][wid] = q; }
+  __syncthreads();
+  if (tid != NT - 1) return;
+  c = r = q = 0.f;
+#pragma unroll
+  for (int k = 0; k < NW; ++k) { c += sum[0][k]; r += sum[1][k]; q += sum[2][k]; }
+  const LikeStat st = {M, c, r, q};
+  like_finish(a, row, st, like_log_total(st), given);
+}
+
+// Joins the chunks of a row: one workgroup per row.  Every wave joins the statistics for itself; the candidates of all chunks (at most 256 x VPT)
+// are selected again.
 template <typename T, int VPT>
 __global__ __launch_bounds__(256) void like_join_kernel(LikeArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[2064];
-  __shared__ LikeStat part[256];
-  const long long row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const float w = a.w ? a.w[row % a.J] : 1.f;
-  LikeStat st = {-INFINITY, 0.f, 0.f, 0.f};
-  for (int c = tid; c < a.chunks; c += 256) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + 4 * (row * a.chunks + c));
-    st = like_join(st, LikeStat{v.x, v.y, v.z, v.w});
-  }
-  part[tid] = st;
-  __syncthreads();
-  for (int o = 128; o; o >>= 1) {
-    if (tid < o) part[tid] = like_join(part[tid], part[tid + o]);
-    __syncthreads();
-  }
-  st = part[0];
-  if (tid == 0) like_finish<T>(a, row, st, w);
-  if (a.K) {
-    const float lt = like_log_total(st);
-    const int n = a.chunks * a.K;
-    float s[VPT];
-    int ix[VPT];
+  __shared__ LikeShared<4> sh;
+  const unsigned row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const float w = a.w ? a.w[row % (unsigned)a.J] : 1.f;
+  const int n = a.chunks * a.K;
+  const float* mrow = a.mask ? a.mask + (long long)(row / (unsigned)a.mask_rows) * a.V : nullptr;
+  const LikeGiven given = like_given<T>(a, a.index ? a.index[row] : -1, reinterpret_cast<const T*>(a.z) + row * a.ldz, mrow, w);
+  const f32x4* part = reinterpret_cast<const f32x4*>(a.part) + (long long)row * a.chunks;
+  float s[VPT];
+  int ix[VPT];
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-      const int at = k * 256 + tid;
-      s[k] = at < n ? a.cand_s[row * n + at] : -INFINITY;
-      ix[k] = at < n ? a.cand_i[row * n + at] : -1;
-    }
-    float* ts = a.top_logp + row * a.K;
-    long long* to = a.top_index + row * a.K;
-    auto index_of = [&](int k) { return ix[k]; };
-    like_select<VPT>(s, index_of, a.K, lds, [&](int r, float v, int i) { ts[r] = i < 0 ? v : (v - st.M) - lt; to[r] = i; });
+  for (int k = 0; k < VPT; ++k) {
+    const int at = min(k * 256 + tid, n - 1);
+    s[k] = n ? a.cand_s[(long long)row * n + at] : -INFINITY;
+    ix[k] = n ? a.cand_i[(long long)row * n + at] : -1;
+    if (k * 256 + tid >= n) s[k] = -INFINITY;
   }
+  float M = -INFINITY;
+  for (int c = lane; c < a.chunks; c += 64) M = fmaxf(M, part[c].x);
+  M = wave_max(M);
+  LikeStat st = {M, 0.f, 0.f, 0.f};
+  for (int c = lane; c < a.chunks; c += 64) {
+    const f32x4 v = part[c];
+    const LikeStat x = like_shift(LikeStat{v.x, v.y, v.z, v.w}, M);
+    st.c += x.c; st.r += x.r; st.q += x.q;
+  }
+  st.c = wave_sum(st.c); st.r = wave_sum(st.r); st.q = wave_sum(st.q);
+  const float lt = like_log_total(st);
+  if (tid == 255) like_finish(a, row, st, lt, given);
+  if (!a.K) return;
+  float own = -INFINITY, m, bound;
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) own = fmaxf(own, s[k]);
+  like_maximum<4>(own, a.K, sh, m, bound);
+  like_push<4, VPT>(sh, s, [&](int k) { return ix[k]; }, own, bound);
+  __syncthreads();
+  float* ts = a.top_logp + (long long)row * a.K;
+  long long* to = a.top_index + (long long)row * a.K;
+  auto index_of = [&](int k) { return ix[k]; };
+  like_select<4, VPT>(s, index_of, a.K, sh, [&](int rk, float v, int i) { ts[rk] = i < 0 ? v : (v - st.M) - lt; to[rk] = i; });
 }
 
 // Rows of at most 512 values: one wave per row, four rows per workgroup, no barrier.
 template <typename T, int VPT>
 __global__ __launch_bounds__(256) void like_fwd_wave_kernel(LikeArgs a) {
   const int lane = threadIdx.x & 63;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const unsigned row = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= a.rows) return;
-  const float w = a.w ? a.w[row % a.J] : 1.f;
+  const float w = a.w ? a.w[row % (unsigned)a.J] : 1.f;
   const T* z = reinterpret_cast<const T*>(a.z) + row * a.ldz;
-  const float* mk = a.mask ? a.mask + (row / a.mask_rows) * a.V : nullptr;
+  const float* mk = a.mask ? a.mask + (long long)(row / (unsigned)a.mask_rows) * a.V : nullptr;
+  const long long t = a.index ? a.index[row] : -1;
   float s[VPT];
   float m = -INFINITY;
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
-    const int i = k * 64 + lane;
-    s[k] = i < a.V && (!mk || mk[i] != 0.f) ? Elem<T>::to_f(z[i]) * w : -INFINITY;
+    const int i = k * 64 + lane, c = min(i, a.V - 1);
+    const float v = Elem<T>::to_f(z[c]) * w, in = mk ? mk[c] : 1.f;
+    s[k] = i < a.V && in != 0.f ? v : -INFINITY;
     m = fmaxf(m, s[k]);
   }
+  const LikeGiven given = like_given<T>(a, t, z, mk, w);
   m = wave_max(m);
   const float m0 = m == -INFINITY ? 0.f : m;
   float c = 0.f, r = 0.f, q = 0.f;
@@ -314,9 +467,9 @@ __global__ __launch_bounds__(256) void like_fwd_wave_kernel(LikeArgs a) {
     if (e != 0.f) q = fmaf(e, d, q);
   }
   const LikeStat st = {m, wave_sum(c), wave_sum(r), wave_sum(q)};
-  if (lane == 0) like_finish<T>(a, row, st, w);
-  if (!a.K) return;
   const float lt = like_log_total(st);
+  if (lane == 0) like_finish(a, row, st, lt, given);
+  if (!a.K) return;
   float last_s = INFINITY;
   int last_i = -1;
   for (int rank = 0; rank < a.K; ++rank) {
@@ -333,7 +486,7 @@ __global__ __launch_bounds__(256) void like_fwd_wave_kernel(LikeArgs a) {
       if (like_before(xs, xi, bs, bi)) { bs = xs; bi = xi; }
     }
     const bool some = bs > -INFINITY;
-    if (lane == 0) { a.top_logp[row * a.K + rank] = some ? (bs - st.M) - lt : bs; a.top_index[row * a.K + rank] = some ? bi : -1; }
+    if (lane == 0) { a.top_logp[(long long)row * a.K + rank] = some ? (bs - st.M) - lt : bs; a.top_index[(long long)row * a.K + rank] = some ? bi : -1; }
     last_s = bs; last_i = bi;
   }
 }
@@ -344,11 +497,13 @@ struct LikeBwdArgs {
   void* gz; float* gw_part; long long rows; int V, chunks;
 };
 
-// dL/ds of one value; what it has to know about its row
+// What dL/ds of a value has to know about its row.
+// dL/dw_j of a row is sum ds z.  The ds add up to 0 -- or to -g where the given pixel has no probability --, so the row's largest logit zr is taken out of
+// every z: what is left of the sum does not cancel, also where the logits are 1e38.
 struct LikeRow { float M, lt, H, g, h, zr; long long t; };
-__device__ __forceinline__ LikeRow like_row(const LikeBwdArgs& a, long long row, float w) {
+__device__ __forceinline__ LikeRow like_row(const LikeBwdArgs& a, unsigned row, float w) {
   LikeRow o;
-  o.M = a.stats[2 * row]; o.lt = a.stats[2 * row + 1];
+  o.M = a.stats[2ll * row]; o.lt = a.stats[2ll * row + 1];
   o.t = a.index ? a.index[row] : -1;
   o.g = a.glogp && o.t >= 0 ? a.glogp[row] : 0.f;
   o.h = a.gentropy ? a.gentropy[row] : 0.f;
@@ -357,100 +512,102 @@ __device__ __forceinline__ LikeRow like_row(const LikeBwdArgs& a, long long row,
   o.zr = w != 0.f && o.M > -INFINITY ? o.M / w : 0.f;              // the logit at the maximum
   return o;
 }
-// dL/dw_j of a row is sum ds z.  The ds add up to 0 -- or to -g where the given pixel has no probability --, so the row's largest logit is taken out
-// of every z: what is left of the sum does not cancel, also where the logits are 1e38.
-__device__ __forceinline__ float like_gw_rest(const LikeRow& o, float st) { return st == -INFINITY && o.g != 0.f && o.M > -INFINITY ? -o.g * o.zr : 0.f; }
-__device__ __forceinline__ float like_ds(const LikeRow& o, float s, bool hit) {
-  if (s == -INFINITY) return 0.f;                                  // no probability: masked, or the row has no pixel at all
+__device__ __forceinline__ float like_ds(const LikeRow& o, float s) {
   const float lp = (s - o.M) - o.lt, p = __expf(lp);
-  const float e = p != 0.f ? o.h * p * (lp + o.H) : 0.f;
-  return o.g * (hit ? -expm1f(lp) : -p) - e;
+  const float ds = -p * (o.g + o.h * (fmaxf(lp, -1e30f) + o.H));
+  return s == -INFINITY ? 0.f : ds;                                // no probability: masked, or the row has no pixel at all
+}
+// ... of the given pixel
+__device__ __forceinline__ float like_ds_given(const LikeRow& o, float s) {
+  const float lp = (s - o.M) - o.lt, p = __expf(lp);
+  return s == -INFINITY ? 0.f : -o.g * expm1f(lp) - p * o.h * (fmaxf(lp, -1e30f) + o.H);
 }
 
+// The gradient, 4096 values of a row per workgroup.  The rows are taken from the last to the first -- the forward pass went the other way, and what it read
+// last is still in the memory-side cache -- and the gradient is stored past the caches, which keep z instead.  Forward and backward of 4096 rows of 50001
+// bf16: 323 us, with both 255 (reading z twice and writing once at copy rate: 249); 5376 rows of 16384 fp32: 205 and 179.
 constexpr int kLikeBwdChunk = 4096;     // 256 threads x 16
-template <typename T, int VPT>
+template <typename T>
 __global__ __launch_bounds__(256) void like_bwd_kernel(LikeBwdArgs a) {
+  constexpr int VPT = kLikeBwdChunk / 256, N = 16 / sizeof(T);
+  typedef __attribute__((ext_vector_type(4), aligned(2))) unsigned Bits;
   __shared__ float red[4];
   const int tid = threadIdx.x;
-  const long long row = (long long)blockIdx.x / a.chunks;
-  const int base = (int)(blockIdx.x - row * a.chunks) * (256 * VPT);
-  const float w = a.w ? a.w[row % a.J] : 1.f;
+  const unsigned block = gridDim.x - 1 - blockIdx.x;
+  const unsigned row = block / (unsigned)a.chunks;
+  // (a last chunk of less than one piece reads what lies before it too, and writes its own)
+  const int chunk = (int)(block - row * (unsigned)a.chunks), first = chunk * kLikeBwdChunk;
+  const int n = min(a.V - first, kLikeBwdChunk), base = n < N ? a.V - N : first, own = first - base, len = n < N ? N : n;
+  const float w = a.w ? a.w[row % (unsigned)a.J] : 1.f;
   const T* z = reinterpret_cast<const T*>(a.z) + row * a.ldz;
-  T* gz = reinterpret_cast<T*>(a.gz) + row * (long long)a.V;
-  const float* mk = a.mask ? a.mask + (row / a.mask_rows) * a.V : nullptr;
-  float v[VPT], mv[VPT];
-#pragma unroll
-  for (int k = 0; k < VPT / 4; ++k) {
-    float t[4];
-    load4(z, base + (k * 256 + tid) * 4, a.V, t, 0.f);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { v[4 * k + e] = t[e]; mv[4 * k + e] = 1.f; }
-  }
-  if (mk) {
-#pragma unroll
-    for (int k = 0; k < VPT / 4; ++k) {
-      float t[4];
-      load4(mk, base + (k * 256 + tid) * 4, a.V, t, 0.f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mv[4 * k + e] = t[e];
-    }
-  }
+  T* gz = reinterpret_cast<T*>(a.gz) + row * (long long)a.V + base;
+  const float* mk = a.mask ? a.mask + (long long)(row / (unsigned)a.mask_rows) * a.V : nullptr;
   const LikeRow o = like_row(a, row, w);
-  float gw = 0.f;
+  float v[VPT], s[VPT];
+  RowPart<T, 256, VPT> part;
+  part.load(z + base, mk ? mk + base : nullptr, len);
+  part.values(mk != nullptr, len, w, v, s);
+  const int t = o.t >= first && o.t < first + n ? (int)(o.t - base) : -1;
+  float gw = 0.f, st = 0.f, vt = 0.f;
+  bool mine = false;
 #pragma unroll
-  for (int k = 0; k < VPT / 4; ++k) {
-    const int i = base + (k * 256 + tid) * 4;
-    Quad<T> q;
+  for (int k = 0; k < VPT; k += N) {
+    const int i = value_index<T, 256>(k);
+    Piece<T> q;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = v[4 * k + e];
-      const float ds = i + e < a.V ? like_ds(o, mv[4 * k + e] == 0.f ? -INFINITY : x * w, i + e == o.t) : 0.f;
-      if (ds != 0.f) gw = fmaf(ds, x - o.zr, gw);
+    for (int e = 0; e < N; ++e) {
+      float ds = like_ds(o, s[k + e]);
       q.v[e] = Elem<T>::from_f(ds * w);
+      if (i + e == t) { mine = true; st = s[k + e]; vt = v[k + e]; ds = 0.f; }
+      if (ds != 0.f && i + e >= own) gw = fmaf(ds, v[k + e] - o.zr, gw);
     }
-    if (i + 3 < a.V) *reinterpret_cast<Quad<T>*>(gz + i) = q;
+    if (i >= own && i + N <= len) __builtin_nontemporal_store(__builtin_bit_cast(Bits, q), reinterpret_cast<Bits*>(gz + i));
     else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i + e < a.V) gz[i + e] = q.v[e];
+      for (int e = 0; e < N; ++e)
+        if (i + e >= own && i + e < len) gz[i + e] = q.v[e];
     }
+  }
+  if (mine) {                                                      // (after its neighbours: the same thread's stores stay in order)
+    const float ds = like_ds_given(o, st);
+    gz[t] = Elem<T>::from_f(ds * w);
+    if (ds != 0.f) gw = fmaf(ds, vt - o.zr, gw);
+    if (o.g != 0.f && st == -INFINITY && o.M > -INFINITY) gw -= o.g * o.zr;
   }
   if (a.gw_part) {
     gw = block_sum1(gw, red);
-    if (tid == 0) {
-      if (base == 0 && o.t >= 0 && o.t < a.V) gw += like_gw_rest(o, mk && mk[o.t] == 0.f ? -INFINITY : Elem<T>::to_f(z[o.t]) * w);
-      a.gw_part[blockIdx.x] = gw;
-    }
+    if (tid == 0) a.gw_part[block] = gw;
   }
 }
 
 template <typename T, int VPT>
 __global__ __launch_bounds__(256) void like_bwd_wave_kernel(LikeBwdArgs a) {
   const int lane = threadIdx.x & 63;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const unsigned row = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= a.rows) return;
-  const float w = a.w ? a.w[row % a.J] : 1.f;
+  const float w = a.w ? a.w[row % (unsigned)a.J] : 1.f;
   const T* z = reinterpret_cast<const T*>(a.z) + row * a.ldz;
   T* gz = reinterpret_cast<T*>(a.gz) + row * (long long)a.V;
-  const float* mk = a.mask ? a.mask + (row / a.mask_rows) * a.V : nullptr;
+  const float* mk = a.mask ? a.mask + (long long)(row / (unsigned)a.mask_rows) * a.V : nullptr;
   const LikeRow o = like_row(a, row, w);
   float gw = 0.f;
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
-    const int i = k * 64 + lane;
+    const int i = k * 64 + lane, c = min(i, a.V - 1);
+    const float x = Elem<T>::to_f(z[c]), s = mk && mk[c] == 0.f ? -INFINITY : x * w;
+    float ds = like_ds(o, s);
+    if (i == o.t) {
+      ds = like_ds_given(o, s);
+      if (o.g != 0.f && s == -INFINITY && o.M > -INFINITY) gw -= o.g * o.zr;
+    }
     if (i < a.V) {
-      const float x = Elem<T>::to_f(z[i]);
-      const float ds = like_ds(o, mk && mk[i] == 0.f ? -INFINITY : x * w, i == o.t);
       if (ds != 0.f) gw = fmaf(ds, x - o.zr, gw);
       gz[i] = Elem<T>::from_f(ds * w);
     }
   }
   if (a.gw_part) {
     gw = wave_sum(gw);
-    if (lane == 0) {
-      if (o.t >= 0 && o.t < a.V) gw += like_gw_rest(o, mk && mk[o.t] == 0.f ? -INFINITY : Elem<T>::to_f(z[o.t]) * w);
-      a.gw_part[row] = gw;
-    }
+    if (lane == 0) a.gw_part[row] = gw;
   }
 }
 
@@ -468,11 +625,11 @@ __global__ __launch_bounds__(256) void like_gw_kernel(const float* __restrict__ 
 
 using namespace pwr;
 
-// Values per workgroup of a row that is split: as many as the registers hold -- but a few long rows do not fill 256 CUs that way, so the chunk is
-// halved (down to 4096 = one wide load per lane and instruction, 16 values per thread) until the launch has 512 workgroups.
+// Values per workgroup of a row that is split: as many as the registers of 512 threads hold -- but a few long rows do not fill 256 CUs that way, so
+// the chunk is halved (down to 4096) until the launch has 256 workgroups.
 static int like_chunk(long long rows, int V) {
   int c = kLikeChunk;
-  while (c > 4096 && rows * ((V + c - 1) / c) < 512) c >>= 1;
+  while (V > c && c > 4096 && rows * ((V + c - 1) / c) < 256) c >>= 1;
   return c;
 }
 static int like_chunks(long long rows, int V) {
@@ -486,7 +643,7 @@ extern "C" size_t pwr_likelihood_workspace_bytes(long long rows, int V, int K) {
   return n == 1 ? 0 : (size_t)rows * n * (16 + 8 * (size_t)K);
 }
 
-template <typename T>
+template <typename T, bool TOP>
 static int like_forward(const LikeArgs& a, hipStream_t s) {
   const long long rows = a.rows;
   if (a.V <= kLikeWaveMax) {
@@ -495,17 +652,25 @@ static int like_forward(const LikeArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((like_fwd_wave_kernel<T, 8>), g, dim3(256), 0, s, a);
     return (int)hipGetLastError();
   }
+  constexpr int N = 16 / sizeof(T);
+  if constexpr (!TOP) {
+    if (a.V > 4096 && (rows >= kLikeWalkRows || a.chunks == 1)) {
+      hipLaunchKernelGGL((like_walk_kernel<T, 256, 16>), dim3((unsigned)rows), dim3(256), 0, s, a);
+      return (int)hipGetLastError();
+    }
+  }
   const dim3 g((unsigned)(rows * a.chunks));
   if (a.chunks == 1) {
-    if (a.V <= 4096) hipLaunchKernelGGL((like_fwd_kernel<T, 16, false>), g, dim3(256), 0, s, a);
-    else if (a.V <= 8192) hipLaunchKernelGGL((like_fwd_kernel<T, 32, false>), g, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((like_fwd_kernel<T, 64, false>), g, dim3(256), 0, s, a);
+    if (a.V <= 256 * N) hipLaunchKernelGGL((like_fwd_kernel<T, 256, N, false, TOP>), g, dim3(256), 0, s, a);
+    else if (a.V <= 1024 * N) hipLaunchKernelGGL((like_fwd_kernel<T, 1024, N, false, TOP>), g, dim3(1024), 0, s, a);
+    else if constexpr (TOP) hipLaunchKernelGGL((like_fwd_kernel<T, 512, 32, false, true>), g, dim3(512), 0, s, a);
     return (int)hipGetLastError();
   }
-  if (a.chunk == 4096) hipLaunchKernelGGL((like_fwd_kernel<T, 16, true>), g, dim3(256), 0, s, a);
-  else if (a.chunk == 8192) hipLaunchKernelGGL((like_fwd_kernel<T, 32, true>), g, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((like_fwd_kernel<T, 64, true>), g, dim3(256), 0, s, a);
-  if (a.chunks * a.K <= 1024) hipLaunchKernelGGL((like_join_kernel<T, 4>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  if (a.chunk <= 1024 * N) hipLaunchKernelGGL((like_fwd_kernel<T, 1024, N, true, TOP>), g, dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((like_fwd_kernel<T, 512, 32, true, TOP>), g, dim3(512), 0, s, a);
+  const int n = a.chunks * a.K;
+  if (n <= 256) hipLaunchKernelGGL((like_join_kernel<T, 1>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  else if (n <= 1024) hipLaunchKernelGGL((like_join_kernel<T, 4>), dim3((unsigned)rows), dim3(256), 0, s, a);
   else hipLaunchKernelGGL((like_join_kernel<T, 16>), dim3((unsigned)rows), dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }
@@ -526,7 +691,9 @@ extern "C" int pwr_likelihood_fwd(const void* z, long long ldz, const float* w, 
     a.cand_s = a.part + 4 * rows * a.chunks;
     a.cand_i = (int*)(a.cand_s + rows * a.chunks * K);
   }
-  return dtype == PWR_F32 ? like_forward<float>(a, (hipStream_t)stream) : like_forward<bf16_t>(a, (hipStream_t)stream);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == PWR_F32) return K ? like_forward<float, true>(a, s) : like_forward<float, false>(a, s);
+  return K ? like_forward<bf16_t, true>(a, s) : like_forward<bf16_t, false>(a, s);
 }
 
 static int like_bwd_chunks(int V) { return V <= kLikeWaveMax ? 1 : (V + kLikeBwdChunk - 1) / kLikeBwdChunk; }
@@ -539,7 +706,7 @@ static void like_backward(const LikeBwdArgs& a, hipStream_t s) {
     const dim3 g((unsigned)((a.rows + 3) / 4));
     if (a.V <= 64) hipLaunchKernelGGL((like_bwd_wave_kernel<T, 1>), g, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((like_bwd_wave_kernel<T, 8>), g, dim3(256), 0, s, a);
-  } else hipLaunchKernelGGL((like_bwd_kernel<T, 16>), dim3((unsigned)(a.rows * a.chunks)), dim3(256), 0, s, a);
+  } else hipLaunchKernelGGL((like_bwd_kernel<T>), dim3((unsigned)(a.rows * a.chunks)), dim3(256), 0, s, a);
 }
 
 extern "C" int pwr_likelihood_bwd(const void* z, long long ldz, const float* w, int J, const float* mask, int mask_rows, const long long* index,

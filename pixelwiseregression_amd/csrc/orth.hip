@@ -33,8 +33,6 @@ typedef __attribute__((ext_vector_type(4))) _Float16 half4;
 
 constexpr float kOrthScale = 4096.f;                     // of every stored pair
 constexpr float kOrthInv = 1.f / 4096.f;
-constexpr int kOrthFlat = 16384;                         // elements per workgroup of the sum of squares
-constexpr int kOrthKS = 32;                              // K per stage of the products
 
 // One matrix.  In a table on the device (a parameter list), or made from the launch's arguments (a batch of equal ones).
 struct OrthItem {
@@ -56,12 +54,6 @@ struct OrthWs {
   __host__ __device__ long long diag(int Mp) const { return 8 * xplane + 8 * aplane; }
   __host__ __device__ long long parts(int Mp) const { return diag(Mp) + 8ll * Mp; }
 };
-static inline int orth_parts(int rows, int cols) { return (int)(((long long)rows * cols + kOrthFlat - 1) / kOrthFlat); }
-static inline long long orth_ws_bytes(int rows, int cols, int Mp, int Np) {
-  const OrthWs w(Mp, Np);
-  return (w.parts(Mp) + 8ll * orth_parts(rows, cols) + 255) / 256 * 256;
-}
-
 struct OrthArgs {
   const OrthItem* items; const int4* tiles;              // table form (items != null): tiles[block] = {item, ti, tj, -}
   OrthItem one; long long src_stride, dst_stride, ws_stride; int per;    // batch form: block = batch * per + tile
@@ -91,26 +83,65 @@ __device__ __forceinline__ void split(float v, half_t& hi, half_t& lo) {
   lo = (half_t)(s - (float)hi);
 }
 
-// ---- what is orthogonalised: a tensor of T with a row stride, or u = g + mu buf of an optimizer step
+// ---- what is orthogonalised: a tensor of T with a row stride, or u = g + mu buf of an optimizer step.  Indices are offsets from the matrix's first
+// element; quad() is four neighbours, at any alignment.
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Quad { T v[4]; };
+
 template <typename T> struct OrthTensor {
   const T* x; long long ld;
-  __device__ __forceinline__ float at(const OrthItem& o, int r, int c) const { return Elem<T>::to_f(x[o.src + (long long)r * ld + c]); }
-  __device__ __forceinline__ float first(const OrthItem& o, int r, int c) const { return at(o, r, c); }
+  __device__ __forceinline__ long long stride(const OrthItem&) const { return ld; }
+  __device__ __forceinline__ float one(const OrthItem& o, long long i) const { return Elem<T>::to_f(x[o.src + i]); }
+  __device__ __forceinline__ void quad(const OrthItem& o, long long i, float (&v)[4]) const {
+    const Quad<T> q = *reinterpret_cast<const Quad<T>*>(x + o.src + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = Elem<T>::to_f(q.v[e]);
+  }
+  __device__ __forceinline__ float first(const OrthItem& o, long long i) const { return one(o, i); }
+  __device__ __forceinline__ void first_quad(const OrthItem& o, long long i, float (&v)[4]) const { quad(o, i, v); }
 };
 struct OrthMomentum {
   const float* g; float* buf; float mu, grad_scale; int nesterov;
-  __device__ __forceinline__ float at(const OrthItem& o, int r, int c) const {
-    const long long i = o.src + (long long)r * o.cols + c;
-    return nesterov ? grad_scale * g[i] + mu * buf[i] : buf[i];
+  __device__ __forceinline__ long long stride(const OrthItem& o) const { return o.cols; }
+  __device__ __forceinline__ float u(float gv, float m) const { return nesterov ? grad_scale * gv + mu * m : m; }
+  __device__ __forceinline__ float one(const OrthItem& o, long long i) const { return u(g[o.src + i], buf[o.src + i]); }
+  __device__ __forceinline__ void quad(const OrthItem& o, long long i, float (&v)[4]) const {
+    const Quad<float> a = *reinterpret_cast<const Quad<float>*>(g + o.src + i), b = *reinterpret_cast<const Quad<float>*>(buf + o.src + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = u(a.v[e], b.v[e]);
   }
   // the first pass over the gradient updates the momentum
-  __device__ __forceinline__ float first(const OrthItem& o, int r, int c) const {
-    const long long i = o.src + (long long)r * o.cols + c;
-    const float gv = grad_scale * g[i], m = mu * buf[i] + gv;
-    buf[i] = m;
-    return nesterov ? gv + mu * m : m;
+  __device__ __forceinline__ float first(const OrthItem& o, long long i) const {
+    const float gv = g[o.src + i], m = mu * buf[o.src + i] + grad_scale * gv;
+    buf[o.src + i] = m;
+    return u(gv, m);
+  }
+  __device__ __forceinline__ void first_quad(const OrthItem& o, long long i, float (&v)[4]) const {
+    const Quad<float> a = *reinterpret_cast<const Quad<float>*>(g + o.src + i);
+    Quad<float> b = *reinterpret_cast<const Quad<float>*>(buf + o.src + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { b.v[e] = mu * b.v[e] + grad_scale * a.v[e]; v[e] = u(a.v[e], b.v[e]); }
+    *reinterpret_cast<Quad<float>*>(buf + o.src + i) = b;
   }
 };
+
+// A matrix's squares are summed by orth_parts() workgroups of orth_part_rows() rows each: about 4096 elements, more where that would be over 1024
+// workgroups (every workgroup of the next launch adds all partial sums).
+__host__ __device__ static inline int orth_part_rows(int rows, int cols) {
+  const long long per = 4096 * (((long long)rows * cols + 4096 * 1024 - 1) / (4096 * 1024));
+  return (int)(per / cols > 1 ? per / cols : 1);
+}
+__host__ __device__ static inline int orth_parts(int rows, int cols) { const int r = orth_part_rows(rows, cols); return (rows + r - 1) / r; }
+static inline long long orth_ws_bytes(int rows, int cols, int Mp, int Np) {
+  const OrthWs w(Mp, Np);
+  return (w.parts(Mp) + 8ll * orth_parts(rows, cols) + 255) / 256 * 256;
+}
+
+__device__ __forceinline__ double orth_block_sum(double s, double* red) {
+  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
 
 // partial sums of squares, in 64 bits: neither 1e30 nor 1e-30 leaves the range, and the norm is exact to its last bit
 template <typename SRC>
@@ -118,56 +149,101 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(OrthArgs g, SRC src) {
   __shared__ double red[4];
   int t; int4 tile;
   const OrthItem o = orth_item(g, t, tile);
-  const int part = t < 0 ? tile.y : t;
-  const long long n = (long long)o.rows * o.cols, base = (long long)part * kOrthFlat;
+  const int part = t < 0 ? tile.y : t, nr = orth_part_rows(o.rows, o.cols), r0 = part * nr, r1 = min(o.rows, r0 + nr);
+  const long long ld = src.stride(o);
+  const bool flat = ld == o.cols;                                   // rows without gaps are one run
   double s = 0.0;
-  for (int k = threadIdx.x; k < kOrthFlat && base + k < n; k += 256) {
-    const long long i = base + k;
-    const int r = (int)(i / o.cols), c = (int)(i - (long long)r * o.cols);
-    const double v = src.first(o, r, c);
-    s += v * v;
+  if (!flat && o.cols < 1024) {                                     // short rows with gaps: 16 threads each
+    for (int r = r0 + (threadIdx.x >> 4); r < r1; r += 16)
+      for (int c = threadIdx.x & 15; c < o.cols; c += 16) {
+        const double v = src.first(o, r * ld + c);
+        s += v * v;
+      }
   }
-  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) reinterpret_cast<double*>(g.ws + o.ws + OrthWs(o.Mp, o.Np).parts(o.Mp))[part] = (red[0] + red[1]) + (red[2] + red[3]);
+  const int runs = flat ? 1 : o.cols < 1024 ? 0 : r1 - r0;
+  const long long len = flat ? (long long)(r1 - r0) * o.cols : o.cols;
+  for (int k = 0; k < runs; ++k) {
+    const long long at = (r0 + k) * ld;
+    long long i = threadIdx.x * 4;
+    for (; i + 3 * 1024 + 4 <= len; i += 4 * 1024) {
+      float v[4][4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) src.first_quad(o, at + i + u * 1024, v[u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += (double)v[u][e] * v[u][e];
+    }
+    for (; i < len; i += 1024) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (i + 4 <= len) src.first_quad(o, at + i, v);
+      else
+        for (int e = 0; i + e < len; ++e) v[e] = src.first(o, at + i + e);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += (double)v[e] * v[e];
+    }
+  }
+  s = orth_block_sum(s, red);
+  if (threadIdx.x == 0) reinterpret_cast<double*>(g.ws + o.ws + OrthWs(o.Mp, o.Np).parts(o.Mp))[part] = s;
 }
 
-// X0 = G / (|G| + eps) as pairs, a 64 x 64 tile per workgroup, transposed where the matrix is tall; zero beyond m x n
+// X0 = G / (|G| + eps) as pairs, a 64 x 64 tile per workgroup, transposed where the matrix is tall; zero beyond m x n.  A thread has four neighbours
+// of a row of the SOURCE in each of four rows 16 apart; its loads are under way while the partial sums are added.
 template <typename SRC>
 __global__ __launch_bounds__(256) void orth_pack_kernel(OrthArgs g, SRC src) {
   __shared__ double red[4];
-  __shared__ float tile_s[64][65];
+  __shared__ float turn[64][65];
   int t; int4 tile;
   const OrthItem o = orth_item(g, t, tile);
   const OrthWs w(o.Mp, o.Np);
   const int tj = t < 0 ? tile.z : t % (o.Np / 64), ti = t < 0 ? tile.y : t / (o.Np / 64);
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int tid = threadIdx.x, a = tid >> 4, b = (tid & 15) * 4;
+  const bool tall = o.rows > o.cols;
+  const int r0 = (tall ? tj : ti) * 64, c0 = (tall ? ti : tj) * 64;
+  const long long ld = src.stride(o);
+  float v[4][4];
+  if (r0 + 64 <= o.rows && c0 + 64 <= o.cols) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) src.quad(o, (r0 + a + 16 * k) * ld + c0 + b, v[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = r0 + a + 16 * k, c = c0 + b + e;
+        const float x = src.one(o, min(r, o.rows - 1) * ld + min(c, o.cols - 1));
+        v[k][e] = r < o.rows && c < o.cols ? x : 0.f;
+      }
+  }
   const double* parts = reinterpret_cast<const double*>(g.ws + o.ws + w.parts(o.Mp));
-  const int np = (int)(((long long)o.rows * o.cols + kOrthFlat - 1) / kOrthFlat);
+  const int np = orth_parts(o.rows, o.cols);
   double s = 0.0;
   for (int k = tid; k < np; k += 256) s += parts[k];
-  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-  if (lane == 0) red[wid] = s;
-  __syncthreads();
-  s = (red[0] + red[1]) + (red[2] + red[3]);
-  const double inv = 1.0 / (sqrt(s) + (double)g.eps);
-  const bool tall = o.rows > o.cols;
-  const int m = tall ? o.cols : o.rows, n = tall ? o.rows : o.cols;
-  // rows of the SOURCE are read along, 64 lanes wide
-  for (int k = wid; k < 64; k += 4) {
-    const int i = ti * 64 + (tall ? lane : k), j = tj * 64 + (tall ? k : lane);
-    const float v = i < m && j < n ? (float)((double)src.at(o, tall ? j : i, tall ? i : j) * inv) : 0.f;
-    tile_s[tall ? lane : k][tall ? k : lane] = v;
+  const double inv = 1.0 / (sqrt(orth_block_sum(s, red)) + (double)g.eps);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[k][e] = (float)((double)v[k][e] * inv);
+  if (tall) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) turn[b + e][a + 16 * k] = v[k][e];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[k][e] = turn[a + 16 * k][b + e];
   }
-  __syncthreads();
   half_t* hi = reinterpret_cast<half_t*>(g.ws + o.ws + w.x(0));
-  half_t* lo = hi + w.xplane;
-  for (int k = wid; k < 64; k += 4) {
-    half_t h, l;
-    split(tile_s[k][lane], h, l);
-    const long long at = (long long)(ti * 64 + k) * o.Np + tj * 64 + lane;
-    hi[at] = h; lo[at] = l;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    half4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { half_t x, y; split(v[k][e], x, y); h[e] = x; l[e] = y; }
+    const long long at = (long long)(ti * 64 + a + 16 * k) * o.Np + tj * 64 + b;
+    *reinterpret_cast<half4*>(hi + at) = h;
+    *reinterpret_cast<half4*>(hi + w.xplane + at) = l;
   }
 }
 
@@ -195,14 +271,19 @@ enum { kGram = 0, kPoly = 1, kApply = 2 };
 // First MFMA operand P: the entries j (a lane ends up with four neighbouring j of one row i), second operand Q: the rows i.
 // A and A A are symmetric: tiles tj >= ti only, written twice.  In B X the columns of X are needed along K: its rows are staged as they are
 // and read transposed by the LDS hardware.
+// TILE 128: stages of 32 along K, two in LDS, the next one in registers on its way.  TILE 64, for the few workgroups of small matrices, where a stage
+// costs its latency: 128 along K in one stage.
 template <int TERMS, int KIND, int TILE, typename OUT>
 __global__ __launch_bounds__(256) void orth_gemm_kernel(OrthArgs g, OUT fin, int last) {
+  constexpr int KS = TILE == 128 ? (TERMS == 3 ? 32 : 64) : 128;        // K per stage
+  constexpr int STAGES = TILE == 128 ? 2 : 1;
   constexpr int HALF = TILE / 2, NF = HALF / 16;                        // 16 x 16 fragments per wave and direction
   constexpr int PLANES = TERMS == 3 ? 2 : 1;
-  constexpr int OPB = TILE * kOrthKS * 2;                               // bytes of one operand plane of a stage
+  constexpr int OPB = TILE * KS * 2;                                    // bytes of one operand plane of a stage
   constexpr int UNITS = OPB / 16 / 256;                                 // 16-byte units per thread and plane
   constexpr int STAGE = 2 * PLANES * OPB;
-  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  constexpr int CK = KS / 8, CT = TILE / 8;                             // 16-byte units of a row along K, and along the tile
+  __shared__ __attribute__((aligned(16))) char lds[STAGES * STAGE];
   int t; int4 tile;
   const OrthItem o = orth_item(g, t, tile);
   const OrthWs w(o.Mp, o.Np);
@@ -225,23 +306,26 @@ __global__ __launch_bounds__(256) void orth_gemm_kernel(OrthArgs g, OUT fin, int
   const half_t* P = KIND == kPoly ? A : X;
   const long long qplane = KIND == kGram ? w.xplane : w.aplane, pplane = KIND == kPoly ? w.aplane : w.xplane;
   const int ldq = KIND == kGram ? o.Np : o.Mp, ldp = KIND == kPoly ? o.Mp : o.Np;
-  const int K = KIND == kGram ? o.Np : o.Mp;
+  const int K = KIND == kGram ? o.Np : o.Mp;                            // a multiple of 64
 
-  // staging: unit u of a plane.  [row][4 chunks of 8] with the chunk swizzled by the row, or (columns of X) [k][TILE] with the 32-byte pieces
-  // swizzled by k, so that neither kind of read meets its own bank
+  // Staging.  A plane is [row][CK units along K], the unit swizzled by the row, or (columns of X) [k][CT units], 32-byte pieces swizzled by k, so
+  // that neither kind of read meets its own bank.  Where K ends inside a stage the units beyond are loaded from inside and not used.
   half8 rq[PLANES][UNITS], rp[PLANES][UNITS];
+  auto ntf = [](int row) { return CK == 4 ? (row >> 1) & 3 : CK == 8 ? (row >> 1) & 7 : row & 15; };
   auto trf = [](int k) { return TILE == 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1; };
   auto load = [&](int k0) {
+    const int left = K - k0;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      const int id = u * 256 + tid;
+      const int id = u * 256 + tid, row = id / CK, c = KS > 64 ? min(id % CK, left / 8 - 1) : id % CK;
+      const int kr = KS > 64 ? min(id / CT, left - 1) : id / CT;
 #pragma unroll
       for (int p = 0; p < PLANES; ++p) {
-        rq[p][u] = *reinterpret_cast<const half8*>(Q + p * qplane + (long long)(ti * TILE + (id >> 2)) * ldq + k0 + (id & 3) * 8);
+        rq[p][u] = *reinterpret_cast<const half8*>(Q + p * qplane + (long long)(ti * TILE + row) * ldq + k0 + c * 8);
         if constexpr (KIND == kApply)
-          rp[p][u] = *reinterpret_cast<const half8*>(P + p * pplane + (long long)(k0 + id / (TILE / 8)) * ldp + tj * TILE + (id % (TILE / 8)) * 8);
+          rp[p][u] = *reinterpret_cast<const half8*>(P + p * pplane + (long long)(k0 + kr) * ldp + tj * TILE + (id % CT) * 8);
         else
-          rp[p][u] = *reinterpret_cast<const half8*>(P + p * pplane + (long long)(tj * TILE + (id >> 2)) * ldp + k0 + (id & 3) * 8);
+          rp[p][u] = *reinterpret_cast<const half8*>(P + p * pplane + (long long)(tj * TILE + row) * ldp + k0 + c * 8);
       }
     }
   };
@@ -250,8 +334,8 @@ __global__ __launch_bounds__(256) void orth_gemm_kernel(OrthArgs g, OUT fin, int
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int id = u * 256 + tid;
-      const int row = id >> 2, nt = row * 64 + (((id & 3) ^ ((row >> 1) & 3)) << 4);
-      const int k = id / (TILE / 8), ch = id % (TILE / 8);
+      const int row = id / CK, nt = row * KS * 2 + (((id % CK) ^ ntf(row)) << 4);
+      const int k = id / CT, ch = id % CT;
       const int tr = k * TILE * 2 + (((ch >> 1) ^ trf(k)) << 5) + ((ch & 1) << 4);
 #pragma unroll
       for (int p = 0; p < PLANES; ++p) {
@@ -260,13 +344,13 @@ __global__ __launch_bounds__(256) void orth_gemm_kernel(OrthArgs g, OUT fin, int
       }
     }
   };
-  auto frag = [&](const char* plane, int row0) {
+  auto frag = [&](const char* plane, int row0, int kk) {
     const int row = row0 + (lane & 15);
-    return *reinterpret_cast<const half8*>(plane + row * 64 + (((lane >> 4) ^ ((row >> 1) & 3)) << 4));
+    return *reinterpret_cast<const half8*>(plane + row * KS * 2 + (((kk * 4 + (lane >> 4)) ^ ntf(row)) << 4));
   };
-  auto frag_tr = [&](const char* plane, int j0) {
+  auto frag_tr = [&](const char* plane, int j0, int kk) {
     typedef __attribute__((address_space(3))) bf16x4* lptr;              // (the read moves 16-bit patterns, whatever they mean)
-    const int i = lane & 15, k = 8 * (lane >> 4) + (i >> 2);
+    const int i = lane & 15, k = kk * 32 + 8 * (lane >> 4) + (i >> 2);
     const char* a0 = plane + k * TILE * 2 + (((j0 >> 4) ^ trf(k)) << 5) + ((i & 3) << 3);
     const half4 lo = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lptr)(a0)));
     const half4 hi = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lptr)(a0 + 4 * TILE * 2)));
@@ -280,23 +364,15 @@ __global__ __launch_bounds__(256) void orth_gemm_kernel(OrthArgs g, OUT fin, int
   for (int p = 0; p < NF; ++p)
 #pragma unroll
     for (int q = 0; q < NF; ++q) acc[p][q] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  load(0);
-  store(0);
-  __syncthreads();
-  int stage = 0;
-  for (int k0 = 0; k0 < K; k0 += kOrthKS) {
-    const bool more = k0 + kOrthKS < K;
-    if (more) load(k0 + kOrthKS);
-    const char* s = lds + stage * STAGE;
+  auto compute = [&](const char* s, int kk) {
     half8 fq[PLANES][NF], fp[PLANES][NF];
 #pragma unroll
     for (int p = 0; p < PLANES; ++p)
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        fq[p][f] = frag(s + p * OPB, wq + 16 * f);
-        if constexpr (KIND == kApply) fp[p][f] = frag_tr(s + (PLANES + p) * OPB, wp + 16 * f);
-        else fp[p][f] = frag(s + (PLANES + p) * OPB, wp + 16 * f);
+        fq[p][f] = frag(s + p * OPB, wq + 16 * f, kk);
+        if constexpr (KIND == kApply) fp[p][f] = frag_tr(s + (PLANES + p) * OPB, wp + 16 * f, kk);
+        else fp[p][f] = frag(s + (PLANES + p) * OPB, wp + 16 * f, kk);
       }
 #pragma unroll
     for (int p = 0; p < NF; ++p)
@@ -308,9 +384,32 @@ __global__ __launch_bounds__(256) void orth_gemm_kernel(OrthArgs g, OUT fin, int
         }
         acc[p][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][p], fq[0][q], acc[p][q], 0, 0, 0);
       }
-    if (more) store(stage ^ 1);
+  };
+
+  load(0);
+  if constexpr (STAGES == 2) {
+    store(0);
     __syncthreads();
-    stage ^= 1;
+    int stage = 0;
+    for (int k0 = 0; k0 < K; k0 += KS) {
+      const bool more = k0 + KS < K;
+      if (more) load(k0 + KS);
+#pragma unroll
+      for (int kk = 0; kk < KS / 32; ++kk) compute(lds + stage * STAGE, kk);
+      if (more) store(stage ^ 1);
+      __syncthreads();
+      stage ^= 1;
+    }
+  } else {
+    for (int k0 = 0; k0 < K; k0 += KS) {
+      if (k0) __syncthreads();                                          // (everyone has read the stage before)
+      store(0);
+      __syncthreads();
+      if (k0 + KS < K) load(k0 + KS);
+#pragma unroll
+      for (int kk = 0; kk < KS / 32; ++kk)
+        if (k0 + kk * 32 < K) compute(lds, kk);
+    }
   }
 
   // epilogue: lane (l & 15) has row i, entries j .. j + 3

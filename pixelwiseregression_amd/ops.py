@@ -124,62 +124,87 @@ class LogLikelihood(NamedTuple):
     top_index: Optional[torch.Tensor]
 
 
+def _plain(t, dtype):
+    """t itself where it is what a kernel reads (a call of these small operators costs its Python), else a copy that is."""
+    if t.dtype is dtype and t.is_contiguous():
+        return t
+    return t.detach().to(dtype).contiguous()
+
+
 class _Rows:
     """The arguments of log_likelihood as the kernels take them: rows of V values, `ld` apart."""
 
+    __slots__ = ("z", "ld", "index", "w", "mask", "mask_rows", "lead", "J", "rows", "V", "dtype")
+
     def __init__(self, z, index, w, mask):
-        if z.dim() not in (2, 3, 4):
-            raise ValueError("z must be [N, V], [B, J, V] or [B, J, H, W], got %s" % (tuple(z.shape),))
+        shape, dim = z.shape, z.dim()
+        if not 2 <= dim <= 4:
+            raise ValueError("z must be [N, V], [B, J, V] or [B, J, H, W], got %s" % (tuple(shape),))
         self.dtype = _dtype_tag(z, "z")
-        self.lead = tuple(z.shape[:1] if z.dim() == 2 else z.shape[:2])
-        self.J = z.shape[1] if z.dim() > 2 else 1
-        v = z.flatten(2) if z.dim() == 4 else z
-        self.rows, self.V = int(torch.Size(self.lead).numel()), v.shape[-1]
+        self.lead = lead = tuple(shape[:1]) if dim == 2 else tuple(shape[:2])
+        self.J = J = shape[1] if dim > 2 else 1
+        v = z.flatten(2) if dim == 4 else z
+        self.rows, self.V = (lead[0] * J if dim > 2 else lead[0]), v.shape[-1]
         if self.V < 1:
             raise ValueError("a row of no values")
-        if self.J < 1:
+        if J < 1:
             raise ValueError("no joints")
-        if (self.V > 1 and v.stride(-1) != 1) or (v.dim() == 3 and v.shape[0] > 1 and self.J > 1 and v.stride(0) != self.J * v.stride(1)):
-            v = v.contiguous()
+        if not v.is_contiguous():
+            if (self.V > 1 and v.stride(-1) != 1) or (v.dim() == 3 and v.shape[0] > 1 and J > 1 and v.stride(0) != J * v.stride(1)):
+                v = v.contiguous()
         self.z = v
-        self.ld = v.stride(1) if v.dim() == 3 and self.J > 1 else v.stride(0)
-        if index is not None:
-            if tuple(index.shape) != self.lead or index.is_floating_point() or index.is_complex() or index.dtype == torch.bool:
-                raise ValueError("index must be whole numbers of shape %s, got %s %s" % (self.lead, index.dtype, tuple(index.shape)))
-            index = index.to(torch.int64).contiguous()
+        self.ld = v.stride(1) if v.dim() == 3 and J > 1 else v.stride(0)
+        dev = z.device
         self.index = index
-        if w is not None:
-            if w.numel() != self.J or not w.is_floating_point():
-                raise ValueError("w must hold one number per joint (%d), got %s" % (self.J, tuple(w.shape)))
-            w = w.detach().reshape(-1).float().contiguous()
+        if index is not None:
+            if index.shape != lead or index.dtype not in _WHOLE:
+                raise ValueError("index must be whole numbers of shape %s, got %s %s" % (lead, index.dtype, tuple(index.shape)))
+            self.index = _plain(index, torch.int64)
+            if index.device != dev:
+                _same_device(z, index)
         self.w = w
+        if w is not None:
+            if w.numel() != J or not w.is_floating_point():
+                raise ValueError("w must hold one number per joint (%d), got %s" % (J, tuple(w.shape)))
+            self.w = _plain(w, torch.float32)
+            if w.device != dev:
+                _same_device(z, w)
         self.mask_rows = 1
-        if mask is not None:
-            m = mask.flatten(2) if z.dim() == 4 and mask.dim() == 4 else mask
-            per_row, per_sample = self.lead + (self.V,), (self.lead[0], 1, self.V)
-            if tuple(m.shape) == per_sample and z.dim() > 2:
-                self.mask_rows = self.J
-            elif tuple(m.shape) != per_row:
-                raise ValueError("mask must be %s or one per sample %s, got %s" % (per_row, per_sample, tuple(mask.shape)))
-            mask = m.detach().float().contiguous()
         self.mask = mask
-        _same_device(z, index, w, mask)
+        if mask is not None:
+            m = mask.flatten(2) if dim == 4 and mask.dim() == 4 else mask
+            if dim > 2 and m.shape == (lead[0], 1, self.V):
+                self.mask_rows = J
+            elif m.shape != lead + (self.V,):
+                raise ValueError("mask must be %s or one per sample %s, got %s" % (lead + (self.V,), (lead[0], 1, self.V), tuple(mask.shape)))
+            self.mask = _plain(m, torch.float32)
+            if mask.device != dev:
+                _same_device(z, mask)
+
+
+_WHOLE = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _likelihood_forward(r, topk, stats):
-    z, dev = r.z, r.z.device
-    logp = torch.empty(r.lead, device=dev, dtype=torch.float32) if r.index is not None else None
-    entropy = torch.empty(r.lead, device=dev, dtype=torch.float32)
-    top_logp = torch.empty(r.lead + (topk,), device=dev, dtype=torch.float32) if topk else None
-    top_index = torch.empty(r.lead + (topk,), device=dev, dtype=torch.int64) if topk else None
-    st = torch.empty(r.rows, 2, device=dev, dtype=torch.float32) if stats else None
+    z, dev, lead = r.z, r.z.device, r.lead
+    if r.index is not None:
+        logp, entropy = torch.empty((2,) + lead, device=dev, dtype=torch.float32).unbind(0)
+    else:
+        logp, entropy = None, torch.empty(lead, device=dev, dtype=torch.float32)
+    top_logp = torch.empty(lead + (topk,), device=dev, dtype=torch.float32) if topk else None
+    top_index = torch.empty(lead + (topk,), device=dev, dtype=torch.int64) if topk else None
+    st = torch.empty((r.rows, 2), device=dev, dtype=torch.float32) if stats else None
     l = _lib.lib()
-    need = l.pwr_likelihood_workspace_bytes(r.rows, r.V, topk)
+    need = l.pwr_likelihood_workspace_bytes(r.rows, r.V, topk) if r.V > 4096 else 0
     ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     with _on(dev):
-        _lib.check(l.pwr_likelihood_fwd(z.data_ptr(), r.ld, _lib.ptr(r.w), r.J, _lib.ptr(r.mask), r.mask_rows, _lib.ptr(r.index), _lib.ptr(logp),
-                                        _lib.ptr(entropy), _lib.ptr(st), _lib.ptr(top_logp), _lib.ptr(top_index), r.rows, r.V, topk, r.dtype,
-                                        _lib.ptr(ws), need, _lib.stream_ptr(dev)), "pwr_likelihood_fwd")
+        _lib.check(l.pwr_likelihood_fwd(z.data_ptr(), r.ld, _ptr(r.w), r.J, _ptr(r.mask), r.mask_rows, _ptr(r.index), _ptr(logp), entropy.data_ptr(),
+                                        _ptr(st), _ptr(top_logp), _ptr(top_index), r.rows, r.V, topk, r.dtype, _ptr(ws), need, _lib.stream_ptr(dev)),
+                   "pwr_likelihood_fwd")
     return logp, entropy, top_logp, top_index, st
 
 
@@ -187,14 +212,14 @@ def _likelihood_backward(r, stats, entropy, glogp, gentropy, need_w):
     dev = r.z.device
     gz = torch.empty(r.z.shape, device=dev, dtype=r.z.dtype)
     gw = torch.empty(r.J, device=dev, dtype=torch.float32) if need_w else None
-    glogp, gentropy = (g.contiguous().float() if g is not None else None for g in (glogp, gentropy))
+    glogp, gentropy = (_plain(g, torch.float32) if g is not None else None for g in (glogp, gentropy))
     l = _lib.lib()
     need = l.pwr_likelihood_bwd_workspace_bytes(r.rows, r.V) if need_w else 0
     ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     with _on(dev):
-        _lib.check(l.pwr_likelihood_bwd(r.z.data_ptr(), r.ld, _lib.ptr(r.w), r.J, _lib.ptr(r.mask), r.mask_rows, _lib.ptr(r.index), stats.data_ptr(),
-                                        entropy.data_ptr(), _lib.ptr(glogp), _lib.ptr(gentropy), gz.data_ptr(), _lib.ptr(gw), r.rows, r.V, r.dtype,
-                                        _lib.ptr(ws), need, _lib.stream_ptr(dev)), "pwr_likelihood_bwd")
+        _lib.check(l.pwr_likelihood_bwd(r.z.data_ptr(), r.ld, _ptr(r.w), r.J, _ptr(r.mask), r.mask_rows, _ptr(r.index), stats.data_ptr(),
+                                        entropy.data_ptr(), _ptr(glogp), _ptr(gentropy), gz.data_ptr(), _ptr(gw), r.rows, r.V, r.dtype, _ptr(ws), need,
+                                        _lib.stream_ptr(dev)), "pwr_likelihood_bwd")
     return gz, gw
 
 
@@ -203,21 +228,24 @@ class LogLikelihoodFn(torch.autograd.Function):
     def forward(ctx, z, w, index, mask, topk):
         r = _Rows(z, index, w, mask)
         logp, entropy, top_logp, top_index, stats = _likelihood_forward(r, topk, True)
-        ctx.save_for_backward(z, w, r.index, r.mask, stats, entropy)
+        ctx.save_for_backward(z, w, stats, entropy)      # (z and w: so that a change of either before the backward pass is noticed)
+        ctx.r = r                                        # inputs and copies of inputs only: no cycle through an output
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*[t for t in (top_logp, top_index) if t is not None])
+        if topk:
+            ctx.mark_non_differentiable(top_logp, top_index)
         return logp, entropy, top_logp, top_index
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, glogp, gentropy, _, __):
-        z, w, index, mask, stats, entropy = ctx.saved_tensors
+        z, w, stats, entropy = ctx.saved_tensors
         if glogp is None and gentropy is None:
-            return (None,) * 5
-        # (mask and index are the kernels' own copies by now: the mask in its row form)
-        r = _Rows(z, index, w, mask)
-        gz, gw = _likelihood_backward(r, stats, entropy, glogp, gentropy, ctx.needs_input_grad[1])
-        return gz.view(z.shape) if ctx.needs_input_grad[0] else None, gw.view(w.shape).to(w.dtype) if gw is not None else None, None, None, None
+            return None, None, None, None, None
+        need_z, need_w = ctx.needs_input_grad[:2]
+        gz, gw = _likelihood_backward(ctx.r, stats, entropy, glogp, gentropy, need_w)
+        if gw is not None and (gw.shape != w.shape or gw.dtype != w.dtype):
+            gw = gw.view(w.shape).to(w.dtype)
+        return (gz if gz.shape == z.shape else gz.view(z.shape)) if need_z else None, gw, None, None, None
 
 
 def log_likelihood(z, index, w=None, mask=None, topk=0):

@@ -90,6 +90,19 @@ def test_lengths(V, dtype):
     check(*inputs(2, 3, V, dtype, w=True, mask="none", seed=V), topk=5)
 
 
+@pytest.mark.parametrize("V", [4099, 8192, 16500, 20481])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", ["none", "sample"])
+def test_many_long_rows(V, dtype, mask):
+    """Enough rows for a workgroup to walk each: the maximum in the first part, in the last, rising from part to part; equal maxima in several parts."""
+    z, index, w, m = inputs(130, 4, V, dtype, mask=mask, seed=V)
+    z[1, 0, 5] = 40.0
+    z[1, 1, V - 1] = 40.0
+    z[1, 2] = torch.linspace(-30, 30, V).to(dtype)
+    z[1, 3, ::4096] = 25.0
+    check(z, index, w, m)
+
+
 @pytest.mark.parametrize("V", [5, 200, 4096, 5000, 20000])
 @pytest.mark.parametrize("mask", ["sample", "row"])
 def test_masks_and_rows_without_a_pixel(V, mask):
