@@ -20,6 +20,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "pwr_common.h"
@@ -55,26 +56,40 @@ struct OrthWs {
   __host__ __device__ long long parts(int Mp) const { return diag(Mp) + 8ll * Mp; }
 };
 struct OrthArgs {
-  const OrthItem* items; const int4* tiles;              // table form (items != null): tiles[block] = {item, ti, tj, -}
-  OrthItem one; long long src_stride, dst_stride, ws_stride; int per;    // batch form: block = batch * per + tile
+  const OrthItem* items; const int4* tiles;              // table form (items != null): tiles[t] = {item, ti, tj, -}
+  OrthItem one; long long src_stride, dst_stride, ws_stride; int per;     // batch form: t = batch * per + tile
   char* ws;
   int buf;                                               // which X buffer is read
   float a, b, c, eps;
+  // a product's tiles from `whole` on are split into `parts` along K: their sums go to slab [tile - whole][part][4 x 4 fragments][256 threads]
+  int whole, parts; f32x4* slab;
 };
 
-__device__ __forceinline__ OrthItem orth_item(const OrthArgs& g, int& t, int4& tile) {
+// the matrix and tile number t of a launch belong to: tile >= 0 is the number within the matrix, else `entry` names it
+__device__ __forceinline__ OrthItem orth_item(const OrthArgs& g, int t, int& tile, int4& entry) {
   if (g.items) {
-    tile = g.tiles[blockIdx.x];
-    t = -1;
-    return g.items[tile.x];
+    entry = g.tiles[t];
+    tile = -1;
+    return g.items[entry.x];
   }
-  const int batch = blockIdx.x / g.per;
-  t = blockIdx.x - batch * g.per;
+  const int batch = t / g.per;
+  tile = t - batch * g.per;
   OrthItem o = g.one;
   o.src += batch * g.src_stride;
   o.dst += batch * g.dst_stride;
   o.ws += batch * g.ws_stride;
   return o;
+}
+// (ti, tj) of a tile of a symmetric product (ti <= tj; column tj starts at number tj (tj + 1) / 2) or of B X
+__device__ __forceinline__ void orth_place(bool symmetric, int tile, const int4& entry, int nj, int& ti, int& tj) {
+  if (tile < 0) { ti = entry.y; tj = entry.z; }
+  else if (!symmetric) { ti = tile / nj; tj = tile - ti * nj; }
+  else {
+    tj = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+    while (tj * (tj + 1) / 2 > tile) --tj;
+    while ((tj + 1) * (tj + 2) / 2 <= tile) ++tj;
+    ti = tile - tj * (tj + 1) / 2;
+  }
 }
 
 __device__ __forceinline__ void split(float v, half_t& hi, half_t& lo) {
@@ -148,7 +163,7 @@ template <typename SRC>
 __global__ __launch_bounds__(256) void orth_norm_kernel(OrthArgs g, SRC src) {
   __shared__ double red[4];
   int t; int4 tile;
-  const OrthItem o = orth_item(g, t, tile);
+  const OrthItem o = orth_item(g, blockIdx.x, t, tile);
   const int part = t < 0 ? tile.y : t, nr = orth_part_rows(o.rows, o.cols), r0 = part * nr, r1 = min(o.rows, r0 + nr);
   const long long ld = src.stride(o);
   const bool flat = ld == o.cols;                                   // rows without gaps are one run
@@ -194,7 +209,7 @@ __global__ __launch_bounds__(256) void orth_pack_kernel(OrthArgs g, SRC src) {
   __shared__ double red[4];
   __shared__ float turn[64][65];
   int t; int4 tile;
-  const OrthItem o = orth_item(g, t, tile);
+  const OrthItem o = orth_item(g, blockIdx.x, t, tile);
   const OrthWs w(o.Mp, o.Np);
   const int tj = t < 0 ? tile.z : t % (o.Np / 64), ti = t < 0 ? tile.y : t / (o.Np / 64);
   const int tid = threadIdx.x, a = tid >> 4, b = (tid & 15) * 4;
@@ -267,36 +282,120 @@ struct OrthNone {
 
 enum { kGram = 0, kPoly = 1, kApply = 2 };
 
-// ---- the products: one TILE x TILE tile of the result per workgroup of four waves, each (TILE / 2)^2.
+// What a finished entry needs besides its sum: the pairs of A (for B) or X (for the next X) at the same place.
+struct OrthPair { half4 h, l; };
+template <int KIND>
+__device__ __forceinline__ OrthPair orth_beside(const OrthArgs& g, const OrthItem& o, const OrthWs& w, int i, int j) {
+  OrthPair r;
+  if constexpr (KIND != kGram) {
+    const char* base = g.ws + o.ws;
+    const half_t* p = reinterpret_cast<const half_t*>(base + (KIND == kPoly ? w.a() : w.x(g.buf))) + (long long)i * (KIND == kPoly ? o.Mp : o.Np) + j;
+    r.h = *reinterpret_cast<const half4*>(p);
+    r.l = *reinterpret_cast<const half4*>(p + (KIND == kPoly ? w.aplane : w.xplane));
+  }
+  return r;
+}
+
+// Four neighbours (i, j .. j + 3) of a finished product, and what becomes of them: A, B or the next X, as pairs; after the last step the result.
+template <int TERMS, int KIND, typename OUT>
+__device__ __forceinline__ void orth_finish(const OrthArgs& g, const OrthItem& o, const OrthWs& w, const OUT& fin, int last, bool mirror, int i, int j,
+                                            const f32x4& acc, const OrthPair& beside) {
+  char* base = g.ws + o.ws;
+  float v[4];
+  half4 h, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = acc[e] * (kOrthInv * kOrthInv);
+  float* dA = reinterpret_cast<float*>(base + w.diag(o.Mp));
+  float* dB = dA + o.Mp;
+  if constexpr (KIND == kApply) {
+    const long long at = (long long)i * o.Np + j;
+    const half4 xh = beside.h, xl = beside.l;
+    const float d = TERMS == 1 ? dB[i] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float xhf = (float)xh[e] * kOrthInv;
+      float r = fmaf(g.a, xhf + (float)xl[e] * kOrthInv, v[e]);
+      if constexpr (TERMS == 1) r = fmaf(d, xhf, r);
+      v[e] = r;
+    }
+    if (last) {
+      const bool tall = o.rows > o.cols;
+      const int m = tall ? o.cols : o.rows, n = tall ? o.rows : o.cols;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i < m && j + e < n) fin.put(o, tall, i, j + e, v[e]);
+    } else {
+      half_t* xo = reinterpret_cast<half_t*>(base + w.x(g.buf ^ 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { half_t a, b; split(v[e], a, b); h[e] = a; l[e] = b; }
+      *reinterpret_cast<half4*>(xo + at) = h;
+      *reinterpret_cast<half4*>(xo + w.xplane + at) = l;
+    }
+  } else {
+    const long long at = (long long)i * o.Mp + j;
+    half_t* dst = reinterpret_cast<half_t*>(base + (KIND == kGram ? w.a() : w.b()));
+    if constexpr (KIND == kPoly) {
+      const half4 ah = beside.h, al = beside.l;
+      const float di = TERMS == 1 ? dA[i] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float aij = ((float)ah[e] + (float)al[e]) * kOrthInv, aa = v[e];
+        if constexpr (TERMS == 1) {
+          if (i == j + e) { aij = di; aa = fmaf(di, di, aa); }
+          else aa = fmaf(di + dA[j + e], aij, aa);
+        }
+        v[e] = fmaf(g.c, aa, g.b * aij);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (TERMS == 1) {
+        if (i == j + e) { (KIND == kGram ? dA : dB)[i] = v[e]; v[e] = 0.f; }
+      }
+      half_t a, b;
+      split(v[e], a, b);
+      h[e] = a; l[e] = b;
+    }
+    *reinterpret_cast<half4*>(dst + at) = h;
+    *reinterpret_cast<half4*>(dst + w.aplane + at) = l;
+    if (mirror) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dst[(long long)(j + e) * o.Mp + i] = h[e];
+        dst[w.aplane + (long long)(j + e) * o.Mp + i] = l[e];
+      }
+    }
+  }
+}
+
+// ---- the products: one TILE x TILE tile of the result per workgroup, four waves by (TILE / 2)^2, KG times over for as many shares of K.
 // First MFMA operand P: the entries j (a lane ends up with four neighbouring j of one row i), second operand Q: the rows i.
 // A and A A are symmetric: tiles tj >= ti only, written twice.  In B X the columns of X are needed along K: its rows are staged as they are
 // and read transposed by the LDS hardware.
-// TILE 128: stages of 32 along K, two in LDS, the next one in registers on its way.  TILE 64, for the few workgroups of small matrices, where a stage
-// costs its latency: 128 along K in one stage.
-template <int TERMS, int KIND, int TILE, typename OUT>
-__global__ __launch_bounds__(256) void orth_gemm_kernel(OrthArgs g, OUT fin, int last) {
+// TILE 128, large matrices: two stages in LDS, the next one in registers on its way; few tiles, or a last round of few, are split along K over workgroups.
+// TILE 64, for the few workgroups of smaller ones, where a stage costs its latency: 128 along K in one stage, its four steps of 32 shared out over KG
+// groups of waves, which add their sums through LDS.
+template <int TERMS, int KIND, int TILE, int KG, typename OUT>
+__global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin, int last) {
+  constexpr int NT = 256 * KG;
   constexpr int KS = TILE == 128 ? (TERMS == 3 ? 32 : 64) : 128;        // K per stage
   constexpr int STAGES = TILE == 128 ? 2 : 1;
   constexpr int HALF = TILE / 2, NF = HALF / 16;                        // 16 x 16 fragments per wave and direction
   constexpr int PLANES = TERMS == 3 ? 2 : 1;
   constexpr int OPB = TILE * KS * 2;                                    // bytes of one operand plane of a stage
-  constexpr int UNITS = OPB / 16 / 256;                                 // 16-byte units per thread and plane
+  constexpr int UNITS = OPB / 16 / NT;                                  // 16-byte units per thread and plane
   constexpr int STAGE = 2 * PLANES * OPB;
   constexpr int CK = KS / 8, CT = TILE / 8;                             // 16-byte units of a row along K, and along the tile
-  __shared__ __attribute__((aligned(16))) char lds[STAGES * STAGE];
-  int t; int4 tile;
-  const OrthItem o = orth_item(g, t, tile);
+  constexpr int SUMS = KG > 1 ? KG * TILE * TILE * 4 : 0;               // the groups' sums
+  __shared__ __attribute__((aligned(16))) char lds[STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS];
+  int t = blockIdx.x, part = 0;
+  const bool split_k = TILE == 128 && t >= g.whole;
+  if (split_k) { const int v = t - g.whole; part = v % g.parts; t = g.whole + v / g.parts; }
+  int tile, ti, tj; int4 entry;
+  const OrthItem o = orth_item(g, t, tile, entry);
   const OrthWs w(o.Mp, o.Np);
-  int ti, tj;
-  if (t < 0) { ti = tile.y; tj = tile.z; }
-  else if (KIND == kApply) { const int nj = o.Np / TILE; ti = t / nj; tj = t - ti * nj; }
-  else {                                                                // t -> (ti <= tj): column tj starts at tj (tj + 1) / 2
-    tj = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-    while (tj * (tj + 1) / 2 > t) --tj;
-    while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
-    ti = t - tj * (tj + 1) / 2;
-  }
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  orth_place(KIND != kApply, tile, entry, o.Np / TILE, ti, tj);
+  const int tid = threadIdx.x, lane = tid & 63, wid = (tid >> 6) & 3, group = tid >> 8;
   const int wp = (wid & 1) * HALF, wq = (wid >> 1) * HALF;              // this wave's part of the tile: entries j, rows i
   char* base = g.ws + o.ws;
   const half_t* X = reinterpret_cast<const half_t*>(base + w.x(g.buf));
@@ -310,37 +409,40 @@ __global__ __launch_bounds__(256) void orth_gemm_kernel(OrthArgs g, OUT fin, int
 
   // Staging.  A plane is [row][CK units along K], the unit swizzled by the row, or (columns of X) [k][CT units], 32-byte pieces swizzled by k, so
   // that neither kind of read meets its own bank.  Where K ends inside a stage the units beyond are loaded from inside and not used.
-  half8 rq[PLANES][UNITS], rp[PLANES][UNITS];
+  constexpr int SETS = STAGES == 1 ? 2 : 1;                             // stages on their way in registers
+  half8 rq[SETS][PLANES][UNITS], rp[SETS][PLANES][UNITS];
+  const bool same = KIND != kApply && ti == tj;                         // both operands are the same rows
+  const int pbase = same ? 0 : PLANES * OPB;
   auto ntf = [](int row) { return CK == 4 ? (row >> 1) & 3 : CK == 8 ? (row >> 1) & 7 : row & 15; };
   auto trf = [](int k) { return TILE == 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1; };
-  auto load = [&](int k0) {
+  auto load = [&](int k0, int set) {
     const int left = K - k0;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      const int id = u * 256 + tid, row = id / CK, c = KS > 64 ? min(id % CK, left / 8 - 1) : id % CK;
+      const int id = u * NT + tid, row = id / CK, c = KS > 64 ? min(id % CK, left / 8 - 1) : id % CK;
       const int kr = KS > 64 ? min(id / CT, left - 1) : id / CT;
 #pragma unroll
       for (int p = 0; p < PLANES; ++p) {
-        rq[p][u] = *reinterpret_cast<const half8*>(Q + p * qplane + (long long)(ti * TILE + row) * ldq + k0 + c * 8);
+        rq[set][p][u] = *reinterpret_cast<const half8*>(Q + p * qplane + (long long)(ti * TILE + row) * ldq + k0 + c * 8);
         if constexpr (KIND == kApply)
-          rp[p][u] = *reinterpret_cast<const half8*>(P + p * pplane + (long long)(k0 + kr) * ldp + tj * TILE + (id % CT) * 8);
-        else
-          rp[p][u] = *reinterpret_cast<const half8*>(P + p * pplane + (long long)(tj * TILE + row) * ldp + k0 + c * 8);
+          rp[set][p][u] = *reinterpret_cast<const half8*>(P + p * pplane + (long long)(k0 + kr) * ldp + tj * TILE + (id % CT) * 8);
+        else if (!same)
+          rp[set][p][u] = *reinterpret_cast<const half8*>(P + p * pplane + (long long)(tj * TILE + row) * ldp + k0 + c * 8);
       }
     }
   };
-  auto store = [&](int stage) {
+  auto store = [&](int stage, int set) {
     char* s = lds + stage * STAGE;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      const int id = u * 256 + tid;
+      const int id = u * NT + tid;
       const int row = id / CK, nt = row * KS * 2 + (((id % CK) ^ ntf(row)) << 4);
       const int k = id / CT, ch = id % CT;
       const int tr = k * TILE * 2 + (((ch >> 1) ^ trf(k)) << 5) + ((ch & 1) << 4);
 #pragma unroll
       for (int p = 0; p < PLANES; ++p) {
-        *reinterpret_cast<half8*>(s + p * OPB + nt) = rq[p][u];
-        *reinterpret_cast<half8*>(s + (PLANES + p) * OPB + (KIND == kApply ? tr : nt)) = rp[p][u];
+        *reinterpret_cast<half8*>(s + p * OPB + nt) = rq[set][p][u];
+        if (!same) *reinterpret_cast<half8*>(s + (PLANES + p) * OPB + (KIND == kApply ? tr : nt)) = rp[set][p][u];
       }
     }
   };
@@ -372,7 +474,7 @@ __global__ __launch_bounds__(256) void orth_gemm_kernel(OrthArgs g, OUT fin, int
       for (int f = 0; f < NF; ++f) {
         fq[p][f] = frag(s + p * OPB, wq + 16 * f, kk);
         if constexpr (KIND == kApply) fp[p][f] = frag_tr(s + (PLANES + p) * OPB, wp + 16 * f, kk);
-        else fp[p][f] = frag(s + (PLANES + p) * OPB, wp + 16 * f, kk);
+        else fp[p][f] = frag(s + pbase + p * OPB, wp + 16 * f, kk);
       }
 #pragma unroll
     for (int p = 0; p < NF; ++p)
@@ -386,105 +488,320 @@ __global__ __launch_bounds__(256) void orth_gemm_kernel(OrthArgs g, OUT fin, int
       }
   };
 
-  load(0);
+  constexpr int OWN = NF * NF / KG;                                     // fragments a group finishes (TILE 64)
+  OrthPair beside[OWN];
+  int kb = 0, ke = K;
+  if (split_k) { const int n = K / KS; kb = n * part / g.parts * KS; ke = n * (part + 1) / g.parts * KS; }
+  const int i0 = ti * TILE + wq + (lane & 15), j0 = tj * TILE + wp + 4 * (lane >> 4);
   if constexpr (STAGES == 2) {
-    store(0);
+    if (kb < ke) { load(kb, 0); store(0, 0); }
     __syncthreads();
     int stage = 0;
-    for (int k0 = 0; k0 < K; k0 += KS) {
-      const bool more = k0 + KS < K;
-      if (more) load(k0 + KS);
+    for (int k0 = kb; k0 < ke; k0 += KS) {
+      const bool more = k0 + KS < ke;
+      if (more) load(k0 + KS, 0);
 #pragma unroll
       for (int kk = 0; kk < KS / 32; ++kk) compute(lds + stage * STAGE, kk);
-      if (more) store(stage ^ 1);
+      if (more) store(stage ^ 1, 0);
       __syncthreads();
       stage ^= 1;
     }
   } else {
-    for (int k0 = 0; k0 < K; k0 += KS) {
-      if (k0) __syncthreads();                                          // (everyone has read the stage before)
-      store(0);
-      __syncthreads();
-      if (k0 + KS < K) load(k0 + KS);
+    load(0, 0);
+    if (KS < K) load(KS, 1);
 #pragma unroll
-      for (int kk = 0; kk < KS / 32; ++kk)
-        if (k0 + kk * 32 < K) compute(lds, kk);
+    for (int k = 0; k < OWN; ++k)
+      beside[k] = orth_beside<KIND>(g, o, w, i0 + 16 * ((group * OWN + k) % NF), j0 + 16 * ((group * OWN + k) / NF));
+    auto turn = [&](int k0, int set) {
+      if (k0) __syncthreads();                                          // (everyone has read the stage before)
+      store(0, set);
+      __syncthreads();
+      if (k0 + 2 * KS < K) load(k0 + 2 * KS, set);
+#pragma unroll
+      for (int kk = 0; kk < KS / 32 / KG; ++kk)
+        if (k0 + (group * (KS / 32 / KG) + kk) * 32 < K) compute(lds, group * (KS / 32 / KG) + kk);
+    };
+    for (int k0 = 0; k0 < K; k0 += 2 * KS) {
+      turn(k0, 0);
+      if (k0 + KS < K) turn(k0 + KS, 1);
     }
   }
 
-  // epilogue: lane (l & 15) has row i, entries j .. j + 3
+  if (split_k) {
+    f32x4* s = g.slab + (long long)(blockIdx.x - g.whole) * (NF * NF * 256);
+#pragma unroll
+    for (int p = 0; p < NF; ++p)
+#pragma unroll
+      for (int q = 0; q < NF; ++q) s[(p * NF + q) * 256 + tid] = acc[p][q];
+    return;
+  }
+  const bool mirror = KIND != kApply && ti != tj;
+  if constexpr (KG == 1) {
+#pragma unroll
+    for (int q = 0; q < NF; ++q)
+#pragma unroll
+      for (int p = 0; p < NF; ++p) {
+        const int i = i0 + 16 * q, j = j0 + 16 * p;
+        orth_finish<TERMS, KIND, OUT>(g, o, w, fin, last, mirror, i, j, acc[p][q], STAGES == 1 ? beside[p * NF + q] : orth_beside<KIND>(g, o, w, i, j));
+      }
+  } else {
+    static_assert(NF * NF % KG == 0, "every group finishes as many fragments");
+    f32x4* s = reinterpret_cast<f32x4*>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < NF; ++p)
+#pragma unroll
+      for (int q = 0; q < NF; ++q) s[((p * NF + q) * KG + group) * 256 + wid * 64 + lane] = acc[p][q];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < OWN; ++k) {
+      const int f = group * OWN + k;
+      f32x4 v = s[f * KG * 256 + wid * 64 + lane];
+#pragma unroll
+      for (int u = 1; u < KG; ++u) v += s[(f * KG + u) * 256 + wid * 64 + lane];
+      orth_finish<TERMS, KIND, OUT>(g, o, w, fin, last, mirror, i0 + 16 * (f % NF), j0 + 16 * (f / NF), v, beside[k]);
+    }
+  }
+}
+
+// the split tiles of a product: a workgroup adds the parts of four of a tile's sixteen fragments and finishes them
+template <int TERMS, int KIND, typename OUT>
+__global__ __launch_bounds__(256) void orth_join_kernel(OrthArgs g, OUT fin, int last) {
+  const int t = blockIdx.x >> 2, p = blockIdx.x & 3, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  int tile, ti, tj; int4 entry;
+  const OrthItem o = orth_item(g, g.whole + t, tile, entry);
+  const OrthWs w(o.Mp, o.Np);
+  orth_place(KIND != kApply, tile, entry, o.Np / 128, ti, tj);
+  const int i0 = ti * 128 + (wid >> 1) * 64 + (lane & 15), j0 = tj * 128 + (wid & 1) * 64 + 16 * p + 4 * (lane >> 4);
+  OrthPair beside[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) beside[q] = orth_beside<KIND>(g, o, w, i0 + 16 * q, j0);
+  const f32x4* s = g.slab + (long long)t * g.parts * 4096 + p * 1024 + tid;
+  f32x4 v[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v[q] = s[q * 256];
+  for (int k = 1; k < g.parts; ++k)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] += s[(long long)k * 4096 + q * 256];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) orth_finish<TERMS, KIND, OUT>(g, o, w, fin, last, KIND != kApply && ti != tj, i0 + 16 * q, j0, v[q], beside[q]);
+}
+
+// ---- small matrices: one workgroup of eight waves does a whole matrix, X in LDS for all steps.  MT x 16 rows (m <= 32 or 64), up to NCAP columns.
+// Every product is the three-product form, for bf16 tensors too: what is left is latency, not arithmetic.
+//   A: a wave pair per quarter of K, each wave half of the 16 x 16 tiles on and above the diagonal; the quarters are added through LDS.
+//   B + a I: two tiles a wave, written over A.      X: a wave takes 16 columns at a time, (B + a I) in registers, and writes them in place.
+template <int MT> struct OrthTri;                       // the tiles (p, q), p <= q, of the two waves of a pair
+template <> struct OrthTri<4> {
+  static constexpr int n[2] = {5, 5}, p[2][5] = {{0, 0, 0, 0, 1}, {1, 1, 2, 2, 3}}, q[2][5] = {{0, 1, 2, 3, 1}, {2, 3, 2, 3, 3}};
+};
+template <> struct OrthTri<2> {
+  static constexpr int n[2] = {2, 1}, p[2][2] = {{0, 0}, {1, 1}}, q[2][2] = {{0, 1}, {1, 1}};
+};
+
+template <int MT, int NCAP, typename SRC, typename OUT>
+__global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OUT fin, int steps) {
+  typedef OrthTri<MT> Tri;
+  constexpr int MP = 16 * MT, KK = MP / 32, TRI = Tri::n[0] + Tri::n[1];
+  constexpr int REGION = 3 * TRI * 1024 > MP * MP * 4 ? 3 * TRI * 1024 : MP * MP * 4;      // A or B, or the quarters' sums
+  __shared__ __attribute__((aligned(16))) char lds[MP * NCAP * 4 + REGION];
+  __shared__ double red[8];
+  int t; int4 tile;
+  const OrthItem o = orth_item(g, blockIdx.x, t, tile);
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, li = lane & 15, lg = lane >> 4;
   const bool tall = o.rows > o.cols;
   const int m = tall ? o.cols : o.rows, n = tall ? o.rows : o.cols;
-  float* dA = reinterpret_cast<float*>(base + w.diag(o.Mp));
-  float* dB = dA + o.Mp;
+  const int NP = (n + 63) & ~63;                        // <= NCAP
+  const int xplane = MP * NP * 2;                       // bytes
+  constexpr int aplane = MP * MP * 2;
+  char* X = lds;
+  char* R = lds + MP * NCAP * 4;
+  // rows are NP * 2 (a multiple of 128) and MP * 2 bytes long, their 16-byte units swizzled by the row
+  const bool odd = (NP & 64) != 0;
+  auto xat = [&](int row, int unit) { return row * NP * 2 + ((unit ^ (odd ? (row >> 1) & 7 : row & 7)) << 4); };
+  auto aat = [&](int row, int unit) { return row * MP * 2 + ((unit ^ ((row >> 1) & (MP / 8 - 1))) << 4); };
+
+  // |G|, then X0: the source is read twice, the second time from the caches
+  for (int k = tid * 16; k < 2 * xplane; k += 512 * 16) *reinterpret_cast<uint4*>(X + k) = uint4{0, 0, 0, 0};
+  const int total = o.rows * o.cols, dr = 512 / o.cols, dc = 512 % o.cols;
+  const long long ld = src.stride(o);
+  auto sweep = [&](auto&& use) {
+    int r = tid / o.cols, c = tid - r * o.cols;
+    for (int base = tid; base - tid < total; base += 8 * 512) {
+      float v[8];
+      int rr[8], cc[8];
 #pragma unroll
-  for (int q = 0; q < NF; ++q) {
-    const int i = ti * TILE + wq + 16 * q + (lane & 15);
+      for (int u = 0; u < 8; ++u) {
+        rr[u] = r; cc[u] = c;
+        v[u] = src.one(o, min(r, o.rows - 1) * ld + c);
+        r += dr; c += dc;
+        if (c >= o.cols) { c -= o.cols; ++r; }
+      }
 #pragma unroll
-    for (int p = 0; p < NF; ++p) {
-      const int j = tj * TILE + wp + 16 * p + 4 * (lane >> 4);
-      half4 h, l;
-      float v[4];
+      for (int u = 0; u < 8; ++u)
+        if (rr[u] < o.rows) use(rr[u], cc[u], v[u]);
+    }
+  };
+  double s = 0.0;
+  sweep([&](int, int, float v) { s += (double)v * v; });
+  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+  if (lane == 0) red[wid] = s;
+  __syncthreads();
+  s = ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
+  const double inv = 1.0 / (sqrt(s) + (double)g.eps);
+  sweep([&](int r, int c, float v) {
+    half_t hi, lo;
+    split((float)((double)v * inv), hi, lo);
+    const int i = tall ? c : r, j = tall ? r : c, at = xat(i, j >> 3) + (j & 7) * 2;
+    *reinterpret_cast<half_t*>(X + at) = hi;
+    *reinterpret_cast<half_t*>(X + xplane + at) = lo;
+  });
+  __syncthreads();
+
+  auto mfma3 = [](const half8 (&p)[2], const half8 (&q)[2], f32x4 acc) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[1], q[0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[0], q[1], acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(p[0], q[0], acc, 0, 0, 0);
+  };
+  auto put4 = [&](char* at, int plane, const float (&v)[4], half4& h, half4& l) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = acc[p][q][e] * (kOrthInv * kOrthInv);
-      if constexpr (KIND == kApply) {
-        const long long at = (long long)i * o.Np + j;
-        const half4 xh = *reinterpret_cast<const half4*>(X + at), xl = *reinterpret_cast<const half4*>(X + w.xplane + at);
-        const float d = TERMS == 1 ? dB[i] : 0.f;
+    for (int e = 0; e < 4; ++e) { half_t a, b; split(v[e], a, b); h[e] = a; l[e] = b; }
+    *reinterpret_cast<half4*>(at) = h;
+    *reinterpret_cast<half4*>(at + plane) = l;
+  };
+  auto gram = [&](auto half) {
+    constexpr int H = decltype(half)::value, NT = Tri::n[H];
+    const int quarter = wid >> 1;
+    f32x4 acc[NT];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float xhf = (float)xh[e] * kOrthInv;
-          float r = fmaf(g.a, xhf + (float)xl[e] * kOrthInv, v[e]);
-          if constexpr (TERMS == 1) r = fmaf(d, xhf, r);
-          v[e] = r;
-        }
-        if (last) {
+    for (int k = 0; k < NT; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int ks = quarter; ks < NP / 32; ks += 4) {
+      half8 f[MT][2];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (i < m && j + e < n) fin.put(o, tall, i, j + e, v[e]);
-        } else {
-          half_t* xo = reinterpret_cast<half_t*>(base + w.x(g.buf ^ 1));
+      for (int r = Tri::p[H][0]; r < MT; ++r)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { half_t a, b; split(v[e], a, b); h[e] = a; l[e] = b; }
-          *reinterpret_cast<half4*>(xo + at) = h;
-          *reinterpret_cast<half4*>(xo + w.xplane + at) = l;
-        }
-      } else {
-        const long long at = (long long)i * o.Mp + j;
-        half_t* dst = reinterpret_cast<half_t*>(base + (KIND == kGram ? w.a() : w.b()));
-        if constexpr (KIND == kPoly) {
-          const half4 ah = *reinterpret_cast<const half4*>(A + at), al = *reinterpret_cast<const half4*>(A + w.aplane + at);
-          const float di = TERMS == 1 ? dA[i] : 0.f;
+        for (int p = 0; p < 2; ++p) f[r][p] = *reinterpret_cast<const half8*>(X + p * xplane + xat(16 * r + li, ks * 4 + lg));
+#pragma unroll
+      for (int k = 0; k < NT; ++k) acc[k] = mfma3(f[Tri::p[H][k]], f[Tri::q[H][k]], acc[k]);
+    }
+    if (quarter) {
+#pragma unroll
+      for (int k = 0; k < NT; ++k) *reinterpret_cast<f32x4*>(R + (((quarter - 1) * TRI + H * Tri::n[0] + k) * 64 + lane) * 16) = acc[k];
+    }
+    __syncthreads();
+    if (!quarter) {
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int u = 0; u < 3; ++u) acc[k] += *reinterpret_cast<const f32x4*>(R + ((u * TRI + H * Tri::n[0] + k) * 64 + lane) * 16);
+    }
+    __syncthreads();
+    if (!quarter) {
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        const int i = 16 * Tri::q[H][k] + li, j = 16 * Tri::p[H][k] + 4 * lg;
+        float v[4];
+        half4 h, l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[k][e] * (kOrthInv * kOrthInv);
+        put4(R + aat(i, j >> 3) + (j & 7) * 2, aplane, v, h, l);
+        if (Tri::p[H][k] != Tri::q[H][k]) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float aij = ((float)ah[e] + (float)al[e]) * kOrthInv, aa = v[e];
-            if constexpr (TERMS == 1) {
-              if (i == j + e) { aij = di; aa = fmaf(di, di, aa); }
-              else aa = fmaf(di + dA[j + e], aij, aa);
-            }
-            v[e] = fmaf(g.c, aa, g.b * aij);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (TERMS == 1) {
-            if (i == j + e) { (KIND == kGram ? dA : dB)[i] = v[e]; v[e] = 0.f; }
-          }
-          half_t a, b;
-          split(v[e], a, b);
-          h[e] = a; l[e] = b;
-        }
-        *reinterpret_cast<half4*>(dst + at) = h;
-        *reinterpret_cast<half4*>(dst + w.aplane + at) = l;
-        if (ti != tj) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            dst[(long long)(j + e) * o.Mp + i] = h[e];
-            dst[w.aplane + (long long)(j + e) * o.Mp + i] = l[e];
+            const int at = aat(j + e, i >> 3) + (i & 7) * 2;
+            *reinterpret_cast<half_t*>(R + at) = h[e];
+            *reinterpret_cast<half_t*>(R + aplane + at) = l[e];
           }
         }
       }
     }
+    __syncthreads();
+  };
+  for (int step = 0; step < steps; ++step) {
+    if (wid & 1) gram(std::integral_constant<int, 1>{});
+    else gram(std::integral_constant<int, 0>{});
+    // B + a I
+    constexpr int PW = MT == 4 ? 2 : 1;
+    const int q = MT == 4 ? wid >> 1 : (wid >> 1) & 1, p0 = MT == 4 ? 2 * (wid & 1) : wid & 1;
+    float v[PW][4];
+    if (MT == 4 || wid < 4) {
+      f32x4 acc[PW];
+#pragma unroll
+      for (int k = 0; k < PW; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        half8 fq[2], fp[PW][2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          fq[p] = *reinterpret_cast<const half8*>(R + p * aplane + aat(16 * q + li, kk * 4 + lg));
+#pragma unroll
+          for (int k = 0; k < PW; ++k) fp[k][p] = *reinterpret_cast<const half8*>(R + p * aplane + aat(16 * (p0 + k) + li, kk * 4 + lg));
+        }
+#pragma unroll
+        for (int k = 0; k < PW; ++k) acc[k] = mfma3(fp[k], fq, acc[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < PW; ++k) {
+        const int i = 16 * q + li, j = 16 * (p0 + k) + 4 * lg, at = aat(i, j >> 3) + (j & 7) * 2;
+        const half4 h = *reinterpret_cast<const half4*>(R + at), l = *reinterpret_cast<const half4*>(R + aplane + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[k][e] = fmaf(g.c, acc[k][e] * (kOrthInv * kOrthInv), g.b * (((float)h[e] + (float)l[e]) * kOrthInv)) + (i == j + e ? g.a : 0.f);
+      }
+    }
+    __syncthreads();
+    if (MT == 4 || wid < 4) {
+#pragma unroll
+      for (int k = 0; k < PW; ++k) {
+        const int i = 16 * q + li, j = 16 * (p0 + k) + 4 * lg;
+        half4 h, l;
+        put4(R + aat(i, j >> 3) + (j & 7) * 2, aplane, v[k], h, l);
+      }
+    }
+    __syncthreads();
+    // X
+    half8 b[KK][MT][2];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int r = 0; r < MT; ++r)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) b[kk][r][p] = *reinterpret_cast<const half8*>(R + p * aplane + aat(16 * r + li, kk * 4 + lg));
+    for (int jb = wid; jb < NP / 16; jb += 8) {
+      f32x4 acc[MT];
+#pragma unroll
+      for (int r = 0; r < MT; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        half8 f[2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          typedef __attribute__((address_space(3))) bf16x4* lptr;
+          const int k = kk * 32 + 8 * lg + (li >> 2), j = jb * 16 + 4 * (li & 3);
+          const half4 lo = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lptr)(X + p * xplane + xat(k, j >> 3) + (j & 7) * 2)));
+          const half4 hi = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lptr)(X + p * xplane + xat(k + 4, j >> 3) + (j & 7) * 2)));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { f[p][e] = lo[e]; f[p][4 + e] = hi[e]; }
+        }
+#pragma unroll
+        for (int r = 0; r < MT; ++r) acc[r] = mfma3(f, b[kk][r], acc[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < MT; ++r) {
+        const int i = 16 * r + li, j = jb * 16 + 4 * lg;
+        float x[4];
+        half4 h, l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = acc[r][e] * (kOrthInv * kOrthInv);
+        if (step < steps - 1) put4(X + xat(i, j >> 3) + (j & 7) * 2, xplane, x, h, l);
+        else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i < m && j + e < n) fin.put(o, tall, i, j + e, x[e]);
+        }
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -520,19 +837,64 @@ static int orth_tile(int rows, int cols, long long batch) {
   return batch * orth_apply_tiles(orth_make(rows, cols, 128), 128) >= 256 ? 128 : 64;
 }
 
-struct OrthCounts { long long flat, pack, sym, apply; };
+// X of such a matrix fits the LDS of one CU
+static bool orth_is_small(int rows, int cols) {
+  const long long m = std::min(rows, cols), n = (std::max(rows, cols) + 63ll) / 64 * 64;
+  return m <= 32 ? n <= 1024 : m <= 64 && n <= 512;
+}
 
+struct OrthCounts { long long n[4]; int gram_k, poly_k; };       // workgroups of the norm, pack, symmetric and B X launches; K of the symmetric ones
+
+// How the tiles of a symmetric product share out over 512 places (two workgroups of 128 x 128 tiles per CU): a launch, or its last round, that fills at
+// most three quarters of them is split along K, into parts of 256 at least.  4096 x 4096, 528 tiles: 16 of them alone cost a round as long as the first.
+struct OrthSplit { int whole, parts; };
+static OrthSplit orth_split(long long tiles, int K) {
+  const long long rest = tiles % 512;
+  const long long parts = rest ? std::min<long long>(512 / rest, K / 256) : 1;
+  if (rest == 0 || rest > 384 || parts < 2) return {(int)tiles, 1};
+  return {(int)(tiles - rest), (int)parts};
+}
+static long long orth_slab_bytes(long long tiles, int gram_k, int poly_k) {
+  long long most = 0;
+  for (const int K : {gram_k, poly_k}) {
+    const OrthSplit s = orth_split(tiles, K);
+    most = std::max(most, (tiles - s.whole) * s.parts * 65536);
+  }
+  return most;
+}
+
+// g.slab: behind the matrices' workspaces
 template <int TERMS, int TILE, typename SRC, typename OUT>
-static int orth_run(OrthArgs g, const OrthCounts& n, const int4* const (&lists)[4], const SRC& src, const OUT& out, int steps, const int (&per)[4],
+static int orth_run(const OrthArgs& g, const OrthCounts& n, const int4* const (&lists)[4], const SRC& src, const OUT& out, int steps, const int (&per)[4],
                     hipStream_t s) {
   const dim3 b(256);
-  auto with = [&](int k, int buf) { OrthArgs h = g; h.tiles = lists[k]; h.per = per[k]; h.buf = buf; return h; };
-  hipLaunchKernelGGL((orth_norm_kernel<SRC>), dim3((unsigned)n.flat), b, 0, s, with(0, 0), src);
-  hipLaunchKernelGGL((orth_pack_kernel<SRC>), dim3((unsigned)n.pack), b, 0, s, with(1, 0), src);
+#ifndef KGS
+#define KGS 4
+#define KGA 4
+#endif
+  constexpr int KG = TILE == 64 ? KGS : 1, KA = TILE == 64 ? KGA : 1;
+  auto with = [&](int k, int buf) { OrthArgs h = g; h.tiles = lists[k]; h.per = per[k]; h.buf = buf; h.whole = 0x7fffffff; h.parts = 1; return h; };
+  hipLaunchKernelGGL((orth_norm_kernel<SRC>), dim3((unsigned)n.n[0]), b, 0, s, with(0, 0), src);
+  hipLaunchKernelGGL((orth_pack_kernel<SRC>), dim3((unsigned)n.n[1]), b, 0, s, with(1, 0), src);
+  auto symmetric = [&](auto kind, int K, int buf) {
+    constexpr int KIND = decltype(kind)::value;
+    OrthArgs h = with(2, buf);
+    long long blocks = n.n[2];
+    if constexpr (TILE == 128) {
+      const OrthSplit sp = orth_split(n.n[2], K);
+      h.whole = sp.whole; h.parts = sp.parts;
+      blocks = sp.whole + (n.n[2] - sp.whole) * sp.parts;
+    }
+    hipLaunchKernelGGL((orth_gemm_kernel<TERMS, KIND, TILE, KG, OrthNone>), dim3((unsigned)blocks), dim3(256 * KG), 0, s, h, OrthNone{}, 0);
+    if constexpr (TILE == 128) {
+      if (h.whole < n.n[2])
+        hipLaunchKernelGGL((orth_join_kernel<TERMS, KIND, OrthNone>), dim3((unsigned)(4 * (n.n[2] - h.whole))), b, 0, s, h, OrthNone{}, 0);
+    }
+  };
   for (int k = 0; k < steps; ++k) {
-    hipLaunchKernelGGL((orth_gemm_kernel<TERMS, kGram, TILE, OrthNone>), dim3((unsigned)n.sym), b, 0, s, with(2, k & 1), OrthNone{}, 0);
-    hipLaunchKernelGGL((orth_gemm_kernel<TERMS, kPoly, TILE, OrthNone>), dim3((unsigned)n.sym), b, 0, s, with(2, k & 1), OrthNone{}, 0);
-    hipLaunchKernelGGL((orth_gemm_kernel<TERMS, kApply, TILE, OUT>), dim3((unsigned)n.apply), b, 0, s, with(3, k & 1), out, k == steps - 1);
+    symmetric(std::integral_constant<int, kGram>{}, n.gram_k, k & 1);
+    symmetric(std::integral_constant<int, kPoly>{}, n.poly_k, k & 1);
+    hipLaunchKernelGGL((orth_gemm_kernel<TERMS, kApply, TILE, KA, OUT>), dim3((unsigned)n.n[3]), dim3(256 * KA), 0, s, with(3, k & 1), out, k == steps - 1);
   }
   return (int)hipGetLastError();
 }
@@ -551,8 +913,10 @@ using namespace pwr;
 
 extern "C" size_t pwr_orthogonalize_workspace_bytes(int rows, int cols, long long batch) {
   if (batch <= 0 || !orth_shape_ok(rows, cols)) return 0;
-  const OrthItem o = orth_make(rows, cols, orth_tile(rows, cols, batch));
-  return (size_t)batch * orth_ws_bytes(rows, cols, o.Mp, o.Np);
+  if (orth_is_small(rows, cols)) return 256;
+  const int tile = orth_tile(rows, cols, batch);
+  const OrthItem o = orth_make(rows, cols, tile);
+  return (size_t)(batch * orth_ws_bytes(rows, cols, o.Mp, o.Np) + (tile == 128 ? orth_slab_bytes(batch * orth_sym_tiles(o, 128), o.Np, o.Mp) : 0));
 }
 
 template <typename T, int TERMS>
@@ -565,14 +929,27 @@ static int orthogonalize(const void* x, long long x_batch, long long x_ld, void*
   g.ws_stride = orth_ws_bytes(rows, cols, g.one.Mp, g.one.Np);
   g.a = a; g.b = b; g.c = c; g.eps = eps;
   const long long per[4] = {orth_parts(rows, cols), (long long)(g.one.Mp / 64) * (g.one.Np / 64), orth_sym_tiles(g.one, tile), orth_apply_tiles(g.one, tile)};
-  const OrthCounts n = {batch * per[0], batch * per[1], batch * per[2], batch * per[3]};
-  if (std::max(std::max(n.flat, n.pack), std::max(n.sym, n.apply)) > 0x7fffffffll) return PWR_EUNSUPPORTED;
+  const OrthCounts n = {{batch * per[0], batch * per[1], batch * per[2], batch * per[3]}, g.one.Np, g.one.Mp};
+  for (const long long k : n.n)
+    if (k > 0x7fffffffll) return PWR_EUNSUPPORTED;
+  g.slab = (f32x4*)(g.ws + batch * g.ws_stride);
   const int4* const lists[4] = {};
   const int iper[4] = {(int)per[0], (int)per[1], (int)per[2], (int)per[3]};
   g.src_stride = x_batch;
   g.dst_stride = (long long)rows * cols;
   const OrthTensor<T> src = {(const T*)x, x_ld};
   const OrthOut<T> dst = {(T*)out, cols};
+  if (orth_is_small(rows, cols)) {
+    if (batch > 0x7fffffffll) return PWR_EUNSUPPORTED;
+    g.per = 1;
+    const dim3 grid((unsigned)batch), block(512);
+    const int m = std::min(rows, cols), np = up(std::max(rows, cols), 64);
+    if (m <= 32 && np <= 256) hipLaunchKernelGGL((orth_small_kernel<2, 256, OrthTensor<T>, OrthOut<T>>), grid, block, 0, s, g, src, dst, steps);
+    else if (m <= 32) hipLaunchKernelGGL((orth_small_kernel<2, 1024, OrthTensor<T>, OrthOut<T>>), grid, block, 0, s, g, src, dst, steps);
+    else if (np <= 128) hipLaunchKernelGGL((orth_small_kernel<4, 128, OrthTensor<T>, OrthOut<T>>), grid, block, 0, s, g, src, dst, steps);
+    else hipLaunchKernelGGL((orth_small_kernel<4, 512, OrthTensor<T>, OrthOut<T>>), grid, block, 0, s, g, src, dst, steps);
+    return (int)hipGetLastError();
+  }
   return tile == 128 ? orth_run<TERMS, 128>(g, n, lists, src, dst, steps, iper, s) : orth_run<TERMS, 64>(g, n, lists, src, dst, steps, iper, s);
 }
 
@@ -595,8 +972,8 @@ namespace {
 
 constexpr int kRestRun = 4096;           // elements per workgroup of the AdamW part
 struct MuonHead {
-  unsigned long long magic, bytes, ws_bytes;
-  int items, tile;
+  unsigned long long magic, bytes, ws_bytes, slab;
+  int items, tile, gram_k, poly_k;
   long long n[4], rest;                  // workgroups of the norm, pack, symmetric and apply launches; of the rest
   long long at_items, at_list[4], at_rest;
 };
@@ -652,8 +1029,11 @@ bool muon_layout(const pwr_muon_param* params, int n, MuonHead& h, std::vector<O
     h.n[1] += (long long)(o.Mp / 64) * (o.Np / 64);
     h.n[2] += orth_sym_tiles(o, h.tile);
     h.n[3] += orth_apply_tiles(o, h.tile);
+    h.gram_k = std::max(h.gram_k, o.Np);
+    h.poly_k = std::max(h.poly_k, o.Mp);
   }
-  h.ws_bytes = ws;
+  h.slab = ws;
+  h.ws_bytes = ws + (h.tile == 128 ? orth_slab_bytes(h.n[2], h.gram_k, h.poly_k) : 0);
   h.rest = (long long)rest.size();
   long long at = (sizeof(MuonHead) + 255) / 256 * 256;
   auto take = [&](long long bytes) { const long long r = at; at += (bytes + 255) / 256 * 256; return r; };
@@ -728,7 +1108,8 @@ extern "C" int pwr_muon_step(const void* plan_host, const void* plan_dev, float*
   ga.items = (const OrthItem*)(d + h->at_items);
   ga.ws = (char*)workspace;
   ga.a = a; ga.b = b; ga.c = c; ga.eps = eps;
-  const OrthCounts n = {h->n[0], h->n[1], h->n[2], h->n[3]};
+  const OrthCounts n = {{h->n[0], h->n[1], h->n[2], h->n[3]}, h->gram_k, h->poly_k};
+  ga.slab = (f32x4*)(ga.ws + h->slab);
   const int4* lists[4];
   for (int k = 0; k < 4; ++k) lists[k] = (const int4*)(d + h->at_list[k]);
   const int4* const (&ls)[4] = lists;

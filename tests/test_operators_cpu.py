@@ -64,8 +64,8 @@ def test_orthogonalize_entry_points_refuse_on_the_host():
     assert orth(rows=2 ** 21) == EUNSUPPORTED and orth(rows=2 ** 16, cols=2 ** 15) == EUNSUPPORTED
     assert orth(ws=None) == ENOSPACE and orth(wsb=100) == ENOSPACE and orth(batch=0) == 0
     assert l.pwr_orthogonalize_workspace_bytes(3, 4, 0) == 0 and l.pwr_orthogonalize_workspace_bytes(2 ** 21, 4, 1) == 0
-    # X twice and A, B as pairs of 16 bits, in tiles of 64
-    assert l.pwr_orthogonalize_workspace_bytes(3, 65, 1) >= (2 * 64 * 128 + 2 * 64 * 64) * 4
+    # X twice and A, B as pairs of 16 bits, in tiles of 64; small matrices live in one workgroup
+    assert l.pwr_orthogonalize_workspace_bytes(70, 130, 1) >= (2 * 128 * 192 + 2 * 128 * 128) * 4 and 0 < l.pwr_orthogonalize_workspace_bytes(3, 65, 1) < 4096
 
 
 def plan(params):
