@@ -282,64 +282,57 @@ struct OrthNone {
 
 enum { kGram = 0, kPoly = 1, kApply = 2 };
 
-// What a finished entry needs besides its sum: the pairs of A (for B) or X (for the next X) at the same place.
-struct OrthPair { half4 h, l; };
-template <int KIND>
-__device__ __forceinline__ OrthPair orth_beside(const OrthArgs& g, const OrthItem& o, const OrthWs& w, int i, int j) {
-  OrthPair r;
+// N neighbouring entries of one row as pairs
+template <int N> struct alignas(N >= 8 ? 16 : 8) Halves { half_t v[N]; };
+template <int N> struct OrthPair { Halves<N> h, l; };
+
+// What finished entries need besides their sums: the pairs of A (for B) or X (for the next X) at the same place.
+template <int KIND, int N>
+__device__ __forceinline__ OrthPair<N> orth_beside(const OrthArgs& g, const OrthItem& o, const OrthWs& w, int i, int j) {
+  OrthPair<N> r;
   if constexpr (KIND != kGram) {
     const char* base = g.ws + o.ws;
     const half_t* p = reinterpret_cast<const half_t*>(base + (KIND == kPoly ? w.a() : w.x(g.buf))) + (long long)i * (KIND == kPoly ? o.Mp : o.Np) + j;
-    r.h = *reinterpret_cast<const half4*>(p);
-    r.l = *reinterpret_cast<const half4*>(p + (KIND == kPoly ? w.aplane : w.xplane));
+    r.h = *reinterpret_cast<const Halves<N>*>(p);
+    r.l = *reinterpret_cast<const Halves<N>*>(p + (KIND == kPoly ? w.aplane : w.xplane));
   }
   return r;
 }
 
-// Four neighbours (i, j .. j + 3) of a finished product, and what becomes of them: A, B or the next X, as pairs; after the last step the result.
-template <int TERMS, int KIND, typename OUT>
-__device__ __forceinline__ void orth_finish(const OrthArgs& g, const OrthItem& o, const OrthWs& w, const OUT& fin, int last, bool mirror, int i, int j,
-                                            const f32x4& acc, const OrthPair& beside) {
+// Entries (i, j .. j + N) of a finished product, and what becomes of them: A, B or the next X, as pairs (returned too); after the last step the result.
+template <int TERMS, int KIND, int N, typename OUT>
+__device__ __forceinline__ OrthPair<N> orth_finish(const OrthArgs& g, const OrthItem& o, const OrthWs& w, const OUT& fin, int last, int i, int j,
+                                                   const float (&sum)[N], const OrthPair<N>& beside) {
   char* base = g.ws + o.ws;
-  float v[4];
-  half4 h, l;
+  float v[N];
+  OrthPair<N> r;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = acc[e] * (kOrthInv * kOrthInv);
+  for (int e = 0; e < N; ++e) v[e] = sum[e] * (kOrthInv * kOrthInv);
   float* dA = reinterpret_cast<float*>(base + w.diag(o.Mp));
   float* dB = dA + o.Mp;
   if constexpr (KIND == kApply) {
-    const long long at = (long long)i * o.Np + j;
-    const half4 xh = beside.h, xl = beside.l;
     const float d = TERMS == 1 ? dB[i] : 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float xhf = (float)xh[e] * kOrthInv;
-      float r = fmaf(g.a, xhf + (float)xl[e] * kOrthInv, v[e]);
-      if constexpr (TERMS == 1) r = fmaf(d, xhf, r);
-      v[e] = r;
+    for (int e = 0; e < N; ++e) {
+      const float xhf = (float)beside.h.v[e] * kOrthInv;
+      float x = fmaf(g.a, xhf + (float)beside.l.v[e] * kOrthInv, v[e]);
+      if constexpr (TERMS == 1) x = fmaf(d, xhf, x);
+      v[e] = x;
     }
     if (last) {
       const bool tall = o.rows > o.cols;
       const int m = tall ? o.cols : o.rows, n = tall ? o.rows : o.cols;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < N; ++e)
         if (i < m && j + e < n) fin.put(o, tall, i, j + e, v[e]);
-    } else {
-      half_t* xo = reinterpret_cast<half_t*>(base + w.x(g.buf ^ 1));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { half_t a, b; split(v[e], a, b); h[e] = a; l[e] = b; }
-      *reinterpret_cast<half4*>(xo + at) = h;
-      *reinterpret_cast<half4*>(xo + w.xplane + at) = l;
+      return r;
     }
   } else {
-    const long long at = (long long)i * o.Mp + j;
-    half_t* dst = reinterpret_cast<half_t*>(base + (KIND == kGram ? w.a() : w.b()));
     if constexpr (KIND == kPoly) {
-      const half4 ah = beside.h, al = beside.l;
       const float di = TERMS == 1 ? dA[i] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float aij = ((float)ah[e] + (float)al[e]) * kOrthInv, aa = v[e];
+      for (int e = 0; e < N; ++e) {
+        float aij = ((float)beside.h.v[e] + (float)beside.l.v[e]) * kOrthInv, aa = v[e];
         if constexpr (TERMS == 1) {
           if (i == j + e) { aij = di; aa = fmaf(di, di, aa); }
           else aa = fmaf(di + dA[j + e], aij, aa);
@@ -347,40 +340,47 @@ __device__ __forceinline__ void orth_finish(const OrthArgs& g, const OrthItem& o
         v[e] = fmaf(g.c, aa, g.b * aij);
       }
     }
+    if constexpr (TERMS == 1) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (TERMS == 1) {
+      for (int e = 0; e < N; ++e)
         if (i == j + e) { (KIND == kGram ? dA : dB)[i] = v[e]; v[e] = 0.f; }
-      }
-      half_t a, b;
-      split(v[e], a, b);
-      h[e] = a; l[e] = b;
     }
-    *reinterpret_cast<half4*>(dst + at) = h;
-    *reinterpret_cast<half4*>(dst + w.aplane + at) = l;
-    if (mirror) {
+  }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        dst[(long long)(j + e) * o.Mp + i] = h[e];
-        dst[w.aplane + (long long)(j + e) * o.Mp + i] = l[e];
-      }
-    }
+  for (int e = 0; e < N; ++e) split(v[e], r.h.v[e], r.l.v[e]);
+  half_t* dst = reinterpret_cast<half_t*>(base + (KIND == kApply ? w.x(g.buf ^ 1) : KIND == kGram ? w.a() : w.b()));
+  const long long at = (long long)i * (KIND == kApply ? o.Np : o.Mp) + j;
+  *reinterpret_cast<Halves<N>*>(dst + at) = r.h;
+  *reinterpret_cast<Halves<N>*>(dst + (KIND == kApply ? w.xplane : w.aplane) + at) = r.l;
+  return r;
+}
+// the same entries on the other side of the diagonal
+template <int KIND, int N>
+__device__ __forceinline__ void orth_mirror(const OrthArgs& g, const OrthItem& o, const OrthWs& w, int i, int j, const OrthPair<N>& r) {
+  half_t* dst = reinterpret_cast<half_t*>(g.ws + o.ws + (KIND == kGram ? w.a() : w.b())) + i;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    dst[(long long)(j + e) * o.Mp] = r.h.v[e];
+    dst[w.aplane + (long long)(j + e) * o.Mp] = r.l.v[e];
   }
 }
 
-// ---- the products: one TILE x TILE tile of the result per workgroup, four waves by (TILE / 2)^2, KG times over for as many shares of K.
-// First MFMA operand P: the entries j (a lane ends up with four neighbouring j of one row i), second operand Q: the rows i.
+// ---- the products: one TILE x TILE tile of the result per workgroup of four waves.
+// First MFMA operand P: the entries j, second operand Q: the rows i.  A lane ends up with four neighbouring j of one row i per fragment; row 4 g + e of
+// fragment p is entry 4 NF g + 4 p + e, so that its NF fragments are 4 NF neighbours, and the 16 x 4 lanes hold whole cache lines.
 // A and A A are symmetric: tiles tj >= ti only, written twice.  In B X the columns of X are needed along K: its rows are staged as they are
 // and read transposed by the LDS hardware.
-// TILE 128, large matrices: two stages in LDS, the next one in registers on its way; few tiles, or a last round of few, are split along K over workgroups.
-// TILE 64, for the few workgroups of smaller ones, where a stage costs its latency: 128 along K in one stage, its four steps of 32 shared out over KG
-// groups of waves, which add their sums through LDS.
+// TILE 128, large matrices: a wave has (TILE / 2)^2; two stages in LDS, the next one in registers on its way; few tiles, or a last round of few, are split
+// along K over workgroups.
+// TILE 64, for the few workgroups of smaller ones, where a stage costs its latency.  B X: stages of 64 along K.  A and A A (KG = 4): stages of 128, two on
+// their way in registers, their four steps of 32 shared out over four groups of four waves, which add their sums through LDS.  (Measured and not kept:
+// fragments straight from memory, no LDS along K, 1.4 to 2 times slower; four waves with the whole tile and a step each, 3 - 8 % slower.)
 template <int TERMS, int KIND, int TILE, int KG, typename OUT>
 __global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin, int last) {
   constexpr int NT = 256 * KG;
-  constexpr int KS = TILE == 128 ? (TERMS == 3 ? 32 : 64) : 128;        // K per stage
+    constexpr int KS = TILE == 128 ? (TERMS == 3 ? 32 : 64) : KG == 4 ? 128 : 64;        // K per stage
   constexpr int STAGES = TILE == 128 ? 2 : 1;
-  constexpr int HALF = TILE / 2, NF = HALF / 16;                        // 16 x 16 fragments per wave and direction
+  constexpr int SIDE = TILE / 2, NF = SIDE / 16;                        // of a wave's part of the tile; 16 x 16 fragments a side
   constexpr int PLANES = TERMS == 3 ? 2 : 1;
   constexpr int OPB = TILE * KS * 2;                                    // bytes of one operand plane of a stage
   constexpr int UNITS = OPB / 16 / NT;                                  // 16-byte units per thread and plane
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin
   const OrthWs w(o.Mp, o.Np);
   orth_place(KIND != kApply, tile, entry, o.Np / TILE, ti, tj);
   const int tid = threadIdx.x, lane = tid & 63, wid = (tid >> 6) & 3, group = tid >> 8;
-  const int wp = (wid & 1) * HALF, wq = (wid >> 1) * HALF;              // this wave's part of the tile: entries j, rows i
+  const int wp = (wid & 1) * SIDE, wq = (wid >> 1) * SIDE;              // this wave's part of the tile: entries j, rows i
   char* base = g.ws + o.ws;
   const half_t* X = reinterpret_cast<const half_t*>(base + w.x(g.buf));
   const half_t* A = reinterpret_cast<const half_t*>(base + w.a());
@@ -407,14 +407,15 @@ __global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin
   const int ldq = KIND == kGram ? o.Np : o.Mp, ldp = KIND == kPoly ? o.Mp : o.Np;
   const int K = KIND == kGram ? o.Np : o.Mp;                            // a multiple of 64
 
-  // Staging.  A plane is [row][CK units along K], the unit swizzled by the row, or (columns of X) [k][CT units], 32-byte pieces swizzled by k, so
-  // that neither kind of read meets its own bank.  Where K ends inside a stage the units beyond are loaded from inside and not used.
-  constexpr int SETS = STAGES == 1 ? 2 : 1;                             // stages on their way in registers
+  // Staging.  A plane is [row][CK units of 16 bytes along K], the unit swizzled by the row, or (columns of X) [k][CT units], swizzled by k: so that the
+  // sixteen rows of a fragment -- neighbours (Q), or four runs of four (P) --, or the four pieces of four rows of a transposing read, meet no bank twice.  Where K ends inside a stage the units beyond are loaded from inside and not used.
+  constexpr int SETS = KG == 4 ? 2 : 1;                             // stages on their way in registers
   half8 rq[SETS][PLANES][UNITS], rp[SETS][PLANES][UNITS];
   const bool same = KIND != kApply && ti == tj;                         // both operands are the same rows
   const int pbase = same ? 0 : PLANES * OPB;
-  auto ntf = [](int row) { return CK == 4 ? (row >> 1) & 3 : CK == 8 ? (row >> 1) & 7 : row & 15; };
-  auto trf = [](int k) { return TILE == 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1; };
+  auto ntq = [](int row) { return CK == 4 ? (row >> 2) & 3 : CK == 8 ? (row >> 1) & 7 : row & 15; };
+  auto ntp = [](int row) { return CK == 4 ? (row >> 4) & 3 : CK == 8 ? ((row >> 1) & 1) | ((row >> 4) & 3) << 1 : (row & 3) | ((row >> 3) & 3) << 2; };
+  auto trf = [](int k) { return TILE == 128 ? (k & 1) << 3 | ((k >> 1) & 1) : ((k >> 1) & 1) << 2; };
   auto load = [&](int k0, int set) {
     const int left = K - k0;
 #pragma unroll
@@ -436,30 +437,35 @@ __global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int id = u * NT + tid;
-      const int row = id / CK, nt = row * KS * 2 + (((id % CK) ^ ntf(row)) << 4);
-      const int k = id / CT, ch = id % CT;
-      const int tr = k * TILE * 2 + (((ch >> 1) ^ trf(k)) << 5) + ((ch & 1) << 4);
+      const int row = id / CK, k = id / CT;
+      const int aq = row * KS * 2 + (((id % CK) ^ ntq(row)) << 4);
+      const int ap = KIND == kApply ? k * TILE * 2 + (((id % CT) ^ trf(k)) << 4) : row * KS * 2 + (((id % CK) ^ ntp(row)) << 4);
 #pragma unroll
       for (int p = 0; p < PLANES; ++p) {
-        *reinterpret_cast<half8*>(s + p * OPB + nt) = rq[set][p][u];
-        if (!same) *reinterpret_cast<half8*>(s + (PLANES + p) * OPB + (KIND == kApply ? tr : nt)) = rp[set][p][u];
+        *reinterpret_cast<half8*>(s + p * OPB + aq) = rq[set][p][u];
+        if (!same) *reinterpret_cast<half8*>(s + (PLANES + p) * OPB + ap) = rp[set][p][u];
       }
     }
   };
-  auto frag = [&](const char* plane, int row0, int kk) {
-    const int row = row0 + (lane & 15);
-    return *reinterpret_cast<const half8*>(plane + row * KS * 2 + (((kk * 4 + (lane >> 4)) ^ ntf(row)) << 4));
+  const int li = lane & 15, lg = lane >> 4;
+  auto frag_q = [&](const char* plane, int f, int kk) {
+    const int row = wq + 16 * f + li;
+    return *reinterpret_cast<const half8*>(plane + row * KS * 2 + (((kk * 4 + lg) ^ ntq(row)) << 4));
   };
-  auto frag_tr = [&](const char* plane, int j0, int kk) {
+  auto frag_p = [&](const char* plane, int f, int kk) {
+    const int row = wp + 4 * NF * (li >> 2) + 4 * f + (li & 3);
+    return *reinterpret_cast<const half8*>(plane + row * KS * 2 + (((kk * 4 + lg) ^ (same ? ntq(row) : ntp(row))) << 4));
+  };
+  auto frag_tr = [&](const char* plane, int f, int kk) {
     typedef __attribute__((address_space(3))) bf16x4* lptr;              // (the read moves 16-bit patterns, whatever they mean)
-    const int i = lane & 15, k = kk * 32 + 8 * (lane >> 4) + (i >> 2);
-    const char* a0 = plane + k * TILE * 2 + (((j0 >> 4) ^ trf(k)) << 5) + ((i & 3) << 3);
+    const int k = kk * 32 + 8 * lg + (li >> 2), j = wp + 4 * NF * (li & 3) + 4 * f;
+    const char* a0 = plane + k * TILE * 2 + (((j >> 3) ^ trf(k)) << 4) + ((j & 4) << 1);
     const half4 lo = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lptr)(a0)));
     const half4 hi = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lptr)(a0 + 4 * TILE * 2)));
-    half8 f;
+    half8 r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { f[e] = lo[e]; f[4 + e] = hi[e]; }
-    return f;
+    for (int e = 0; e < 4; ++e) { r[e] = lo[e]; r[4 + e] = hi[e]; }
+    return r;
   };
   f32x4 acc[NF][NF];
 #pragma unroll
@@ -472,9 +478,9 @@ __global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin
     for (int p = 0; p < PLANES; ++p)
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        fq[p][f] = frag(s + p * OPB, wq + 16 * f, kk);
-        if constexpr (KIND == kApply) fp[p][f] = frag_tr(s + (PLANES + p) * OPB, wp + 16 * f, kk);
-        else fp[p][f] = frag(s + pbase + p * OPB, wp + 16 * f, kk);
+        fq[p][f] = frag_q(s + p * OPB, f, kk);
+        if constexpr (KIND == kApply) fp[p][f] = frag_tr(s + (PLANES + p) * OPB, f, kk);
+        else fp[p][f] = frag_p(s + pbase + p * OPB, f, kk);
       }
 #pragma unroll
     for (int p = 0; p < NF; ++p)
@@ -488,11 +494,14 @@ __global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin
       }
   };
 
-  constexpr int OWN = NF * NF / KG;                                     // fragments a group finishes (TILE 64)
-  OrthPair beside[OWN];
+  // a group finishes ROWS fragment rows (16 rows i) of 4 NP neighbours
+  constexpr int NP = NF * NF / KG < NF ? NF * NF / KG : NF, ROWS = NF * NF / KG / NP;
+  static_assert(NP * ROWS * KG == NF * NF, "every group finishes as many fragments");
+  const int q0 = NP < NF ? group * NP / NF : group * ROWS, p0 = NP < NF ? group * NP % NF : 0;
+  OrthPair<4 * NP> beside[ROWS];
   int kb = 0, ke = K;
   if (split_k) { const int n = K / KS; kb = n * part / g.parts * KS; ke = n * (part + 1) / g.parts * KS; }
-  const int i0 = ti * TILE + wq + (lane & 15), j0 = tj * TILE + wp + 4 * (lane >> 4);
+  const int i0 = ti * TILE + wq + 16 * q0 + li, j0 = tj * TILE + wp + 4 * NF * lg + 4 * p0;
   if constexpr (STAGES == 2) {
     if (kb < ke) { load(kb, 0); store(0, 0); }
     __syncthreads();
@@ -508,22 +517,21 @@ __global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin
     }
   } else {
     load(0, 0);
-    if (KS < K) load(KS, 1);
+    if (SETS == 2 && KS < K) load(KS, SETS - 1);
 #pragma unroll
-    for (int k = 0; k < OWN; ++k)
-      beside[k] = orth_beside<KIND>(g, o, w, i0 + 16 * ((group * OWN + k) % NF), j0 + 16 * ((group * OWN + k) / NF));
+    for (int r = 0; r < ROWS; ++r) beside[r] = orth_beside<KIND, 4 * NP>(g, o, w, i0 + 16 * r, j0);
     auto turn = [&](int k0, int set) {
       if (k0) __syncthreads();                                          // (everyone has read the stage before)
       store(0, set);
       __syncthreads();
-      if (k0 + 2 * KS < K) load(k0 + 2 * KS, set);
+      if (k0 + SETS * KS < K) load(k0 + SETS * KS, set);
 #pragma unroll
       for (int kk = 0; kk < KS / 32 / KG; ++kk)
         if (k0 + (group * (KS / 32 / KG) + kk) * 32 < K) compute(lds, group * (KS / 32 / KG) + kk);
     };
-    for (int k0 = 0; k0 < K; k0 += 2 * KS) {
+    for (int k0 = 0; k0 < K; k0 += SETS * KS) {
       turn(k0, 0);
-      if (k0 + KS < K) turn(k0 + KS, 1);
+      if (SETS == 2 && k0 + KS < K) turn(k0 + KS, SETS - 1);
     }
   }
 
@@ -536,55 +544,93 @@ __global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin
     return;
   }
   const bool mirror = KIND != kApply && ti != tj;
-  if constexpr (KG == 1) {
-#pragma unroll
-    for (int q = 0; q < NF; ++q)
-#pragma unroll
-      for (int p = 0; p < NF; ++p) {
-        const int i = i0 + 16 * q, j = j0 + 16 * p;
-        orth_finish<TERMS, KIND, OUT>(g, o, w, fin, last, mirror, i, j, acc[p][q], STAGES == 1 ? beside[p * NF + q] : orth_beside<KIND>(g, o, w, i, j));
-      }
-  } else {
-    static_assert(NF * NF % KG == 0, "every group finishes as many fragments");
-    f32x4* s = reinterpret_cast<f32x4*>(lds);
+  f32x4* sums = reinterpret_cast<f32x4*>(lds);
+  if constexpr (KG > 1) {
     __syncthreads();
 #pragma unroll
     for (int p = 0; p < NF; ++p)
 #pragma unroll
-      for (int q = 0; q < NF; ++q) s[((p * NF + q) * KG + group) * 256 + wid * 64 + lane] = acc[p][q];
+      for (int q = 0; q < NF; ++q) sums[((p * NF + q) * KG + group) * 256 + wid * 64 + lane] = acc[p][q];
     __syncthreads();
+  }
+  // (the tile's other side: a wave's 64 x 64 block goes through LDS, where the transposing reads make 16 bytes along i of it)
+  char* turn = lds + (wid & 3) * 16384;
 #pragma unroll
-    for (int k = 0; k < OWN; ++k) {
-      const int f = group * OWN + k;
-      f32x4 v = s[f * KG * 256 + wid * 64 + lane];
+  for (int r = 0; r < ROWS; ++r) {
+    float v[4 * NP];
 #pragma unroll
-      for (int u = 1; u < KG; ++u) v += s[(f * KG + u) * 256 + wid * 64 + lane];
-      orth_finish<TERMS, KIND, OUT>(g, o, w, fin, last, mirror, i0 + 16 * (f % NF), j0 + 16 * (f / NF), v, beside[k]);
+    for (int k = 0; k < NP; ++k) {
+      f32x4 a = acc[k][r];
+      if constexpr (KG > 1) {
+        const int f = (p0 + k) * NF + q0 + r;
+        a = sums[f * KG * 256 + wid * 64 + lane];
+#pragma unroll
+        for (int u = 1; u < KG; ++u) a += sums[(f * KG + u) * 256 + wid * 64 + lane];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * k + e] = a[e];
+    }
+    const int i = i0 + 16 * r;
+    const OrthPair<4 * NP> b = STAGES == 1 ? beside[r] : orth_beside<KIND, 4 * NP>(g, o, w, i, j0);
+    const OrthPair<4 * NP> d = orth_finish<TERMS, KIND, 4 * NP, OUT>(g, o, w, fin, last, i, j0, v, b);
+    if (!mirror) continue;
+    if constexpr (TILE == 128) {
+      // row i of the block: 128 bytes per plane, its 16-byte units swizzled
+      const int row = 16 * r + li;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int at = row * 128 + (((2 * lg + k) ^ ((row >> 1) & 7)) << 4);
+        *reinterpret_cast<Halves<8>*>(turn + at) = *reinterpret_cast<const Halves<8>*>(d.h.v + 8 * k);
+        *reinterpret_cast<Halves<8>*>(turn + 8192 + at) = *reinterpret_cast<const Halves<8>*>(d.l.v + 8 * k);
+      }
+    } else orth_mirror<KIND, 4 * NP>(g, o, w, i, j0, d);
+  }
+  if constexpr (TILE == 128 && KIND != kApply) {
+    if (mirror) {                                                       // (a wave's own block: its reads follow its writes)
+      typedef __attribute__((address_space(3))) bf16x4* lptr;
+      half_t* dst = reinterpret_cast<half_t*>(base + (KIND == kGram ? w.a() : w.b()));
+#pragma unroll
+      for (int plane = 0; plane < 2; ++plane)
+#pragma unroll
+        for (int jb = 0; jb < 4; ++jb)
+#pragma unroll
+          for (int ib = 0; ib < 2; ++ib) {
+            // lane (lg, li): entry jb 16 + li of the rows ib 32 + 8 lg ... + 7
+            const int row = ib * 32 + 8 * lg + (li >> 2), j = jb * 16 + 4 * (li & 3);
+            auto at = [&](int r) { return turn + plane * 8192 + r * 128 + (((j >> 3) ^ ((r >> 1) & 7)) << 4) + ((j & 4) << 1); };
+            const half4 lo = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lptr)at(row)));
+            const half4 hi = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lptr)at(row + 4)));
+            half8 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[e] = lo[e]; x[4 + e] = hi[e]; }
+            *reinterpret_cast<half8*>(dst + plane * w.aplane + (long long)(tj * TILE + wp + jb * 16 + li) * o.Mp + ti * TILE + wq + ib * 32 + 8 * lg) = x;
+          }
     }
   }
 }
 
-// the split tiles of a product: a workgroup adds the parts of four of a tile's sixteen fragments and finishes them
+// the split tiles of a product: a workgroup adds the parts of one of a tile's four fragment rows and finishes it
 template <int TERMS, int KIND, typename OUT>
 __global__ __launch_bounds__(256) void orth_join_kernel(OrthArgs g, OUT fin, int last) {
-  const int t = blockIdx.x >> 2, p = blockIdx.x & 3, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int t = blockIdx.x >> 2, q = blockIdx.x & 3, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   int tile, ti, tj; int4 entry;
   const OrthItem o = orth_item(g, g.whole + t, tile, entry);
   const OrthWs w(o.Mp, o.Np);
   orth_place(KIND != kApply, tile, entry, o.Np / 128, ti, tj);
-  const int i0 = ti * 128 + (wid >> 1) * 64 + (lane & 15), j0 = tj * 128 + (wid & 1) * 64 + 16 * p + 4 * (lane >> 4);
-  OrthPair beside[4];
+  const int i = ti * 128 + (wid >> 1) * 64 + 16 * q + (lane & 15), j = tj * 128 + (wid & 1) * 64 + 16 * (lane >> 4);
+  const OrthPair<16> beside = orth_beside<KIND, 16>(g, o, w, i, j);
+  const f32x4* s = g.slab + (long long)t * g.parts * 4096 + q * 256 + tid;
+  f32x4 a[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) beside[q] = orth_beside<KIND>(g, o, w, i0 + 16 * q, j0);
-  const f32x4* s = g.slab + (long long)t * g.parts * 4096 + p * 1024 + tid;
-  f32x4 v[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) v[q] = s[q * 256];
+  for (int p = 0; p < 4; ++p) a[p] = s[p * 1024];
   for (int k = 1; k < g.parts; ++k)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] += s[(long long)k * 4096 + q * 256];
+    for (int p = 0; p < 4; ++p) a[p] += s[(long long)k * 4096 + p * 1024];
+  float v[16];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) orth_finish<TERMS, KIND, OUT>(g, o, w, fin, last, KIND != kApply && ti != tj, i0 + 16 * q, j0, v[q], beside[q]);
+  for (int e = 0; e < 16; ++e) v[e] = a[e / 4][e % 4];
+  const OrthPair<16> d = orth_finish<TERMS, KIND, 16, OUT>(g, o, w, fin, last, i, j, v, beside);
+  if (KIND != kApply && ti != tj) orth_mirror<KIND, 16>(g, o, w, i, j, d);
 }
 
 // ---- small matrices: one workgroup of eight waves does a whole matrix, X in LDS for all steps.  MT x 16 rows (m <= 32 or 64), up to NCAP columns.
@@ -832,9 +878,11 @@ static OrthItem orth_make(int rows, int cols, int tile) {
 static long long orth_sym_tiles(const OrthItem& o, int tile) { const long long t = o.Mp / tile; return t * (t + 1) / 2; }
 static long long orth_apply_tiles(const OrthItem& o, int tile) { return (long long)(o.Mp / tile) * (o.Np / tile); }
 
-// 128 x 128 tiles move half the bytes per product of 64 x 64 ones, but a launch of them fills the chip only from 256 tiles on
+// 128 x 128 tiles move half the bytes per product of 64 x 64 ones; they pay from three tiles a side on, where a launch of them has a workgroup per CU.  One
+// matrix in 128 / 64: 2048 x 2048 fp32 835 / 1020 us, 700 x 7000 475 / 583, 1024 x 4096 469 / 475, 1024 x 2048 398 / 307; 64 of 128 x 1152 341 / 283.
+constexpr int kOrthWideSide = 384, kOrthWideTiles = 256;
 static int orth_tile(int rows, int cols, long long batch) {
-  return batch * orth_apply_tiles(orth_make(rows, cols, 128), 128) >= 256 ? 128 : 64;
+  return std::min(rows, cols) >= kOrthWideSide && batch * orth_apply_tiles(orth_make(rows, cols, 128), 128) >= kOrthWideTiles ? 128 : 64;
 }
 
 // X of such a matrix fits the LDS of one CU
@@ -868,11 +916,7 @@ template <int TERMS, int TILE, typename SRC, typename OUT>
 static int orth_run(const OrthArgs& g, const OrthCounts& n, const int4* const (&lists)[4], const SRC& src, const OUT& out, int steps, const int (&per)[4],
                     hipStream_t s) {
   const dim3 b(256);
-#ifndef KGS
-#define KGS 4
-#define KGA 4
-#endif
-  constexpr int KG = TILE == 64 ? KGS : 1, KA = TILE == 64 ? KGA : 1;
+  constexpr int KG = TILE == 64 ? 4 : 1;
   auto with = [&](int k, int buf) { OrthArgs h = g; h.tiles = lists[k]; h.per = per[k]; h.buf = buf; h.whole = 0x7fffffff; h.parts = 1; return h; };
   hipLaunchKernelGGL((orth_norm_kernel<SRC>), dim3((unsigned)n.n[0]), b, 0, s, with(0, 0), src);
   hipLaunchKernelGGL((orth_pack_kernel<SRC>), dim3((unsigned)n.n[1]), b, 0, s, with(1, 0), src);
@@ -894,7 +938,7 @@ static int orth_run(const OrthArgs& g, const OrthCounts& n, const int4* const (&
   for (int k = 0; k < steps; ++k) {
     symmetric(std::integral_constant<int, kGram>{}, n.gram_k, k & 1);
     symmetric(std::integral_constant<int, kPoly>{}, n.poly_k, k & 1);
-    hipLaunchKernelGGL((orth_gemm_kernel<TERMS, kApply, TILE, KA, OUT>), dim3((unsigned)n.n[3]), dim3(256 * KA), 0, s, with(3, k & 1), out, k == steps - 1);
+    hipLaunchKernelGGL((orth_gemm_kernel<TERMS, kApply, TILE, 1, OUT>), dim3((unsigned)n.n[3]), b, 0, s, with(3, k & 1), out, k == steps - 1);
   }
   return (int)hipGetLastError();
 }
@@ -979,17 +1023,17 @@ struct MuonHead {
 };
 constexpr unsigned long long kMuonMagic = 0x31304e4f554d5750ull;
 
-// what the launches of a list cost with a tile: the padded products, in units of one product of a 64 x 64 x 64 block
-long long muon_cost(const std::vector<OrthItem>& v, int tile, long long* blocks) {
-  long long c = 0;
-  *blocks = 0;
+// a list is worked on in the tile that most of its products want (in units of a 64 x 64 x 64 block): the rule of orth_tile
+int muon_tile(const std::vector<OrthItem>& v) {
+  double wide = 0, all = 0;
+  long long tiles = 0;
   for (const OrthItem& k : v) {
-    const OrthItem o = orth_make(k.rows, k.cols, tile);
-    const long long m = o.Mp / 64, n = o.Np / 64;
-    c += m * m * (2 * n + m);
-    *blocks += orth_apply_tiles(o, tile);
+    const OrthItem o = orth_make(k.rows, k.cols, 64);
+    const double m = o.Mp / 64, n = o.Np / 64, c = m * m * (2 * n + m);
+    all += c;
+    if (std::min(k.rows, k.cols) >= kOrthWideSide) { wide += c; tiles += orth_apply_tiles(orth_make(k.rows, k.cols, 128), 128); }
   }
-  return c;
+  return 2 * wide >= all && tiles >= kOrthWideTiles ? 128 : 64;
 }
 
 bool muon_layout(const pwr_muon_param* params, int n, MuonHead& h, std::vector<OrthItem>& items, std::vector<longlong2>& rest) {
@@ -1014,10 +1058,7 @@ bool muon_layout(const pwr_muon_param* params, int n, MuonHead& h, std::vector<O
   memset(&h, 0, sizeof h);
   h.magic = kMuonMagic;
   h.items = (int)items.size();
-  // (the rule of orth_tile, and no wide tile where its padding costs over a quarter more)
-  long long b64, b128;
-  const long long c64 = muon_cost(items, 64, &b64), c128 = muon_cost(items, 128, &b128);
-  h.tile = b128 >= 256 && 4 * c128 <= 5 * c64 ? 128 : 64;
+  h.tile = muon_tile(items);
   long long ws = 0;
   for (OrthItem& o : items) {
     const OrthItem q = orth_make(o.rows, o.cols, h.tile);
