@@ -80,16 +80,29 @@ __device__ __forceinline__ OrthItem orth_item(const OrthArgs& g, int t, int& til
   o.ws += batch * g.ws_stride;
   return o;
 }
-// (ti, tj) of a tile of a symmetric product (ti <= tj; column tj starts at number tj (tj + 1) / 2) or of B X
-__device__ __forceinline__ void orth_place(bool symmetric, int tile, const int4& entry, int nj, int& ti, int& tj) {
+// (ti, tj) of a tile of B X, or of a symmetric product: ti <= tj, in blocks of 4 x 4 tiles, block column J from tile 2 J (4 J + 1) on: workgroups that run
+// together on a chip die read few different rows.  T: tiles a side; nj: tiles a row of X.
+__device__ __forceinline__ void orth_place(bool symmetric, int tile, const int4& entry, int T, int nj, int& ti, int& tj) {
   if (tile < 0) { ti = entry.y; tj = entry.z; }
   else if (!symmetric) { ti = tile / nj; tj = tile - ti * nj; }
   else {
-    tj = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-    while (tj * (tj + 1) / 2 > tile) --tj;
-    while ((tj + 1) * (tj + 2) / 2 <= tile) ++tj;
-    ti = tile - tj * (tj + 1) / 2;
+    int J = (int)((sqrtf(4.f + 32.f * tile) - 2.f) * (1.f / 16.f));
+    while (2 * J * (4 * J + 1) > tile) --J;
+    while (2 * (J + 1) * (4 * J + 5) <= tile) ++J;
+    const int wide = min(4, T - 4 * J), rest = tile - 2 * J * (4 * J + 1), I = min(rest / (4 * wide), J), in = rest - I * 4 * wide;
+    if (I < J) { ti = 4 * I + in / wide; tj = 4 * J + in % wide; }
+    else {
+      int c = 0;
+      while ((c + 1) * (c + 2) / 2 <= in) ++c;
+      tj = 4 * J + c;
+      ti = 4 * J + in - c * (c + 1) / 2;
+    }
   }
+}
+// Workgroup b of n, dealt round over the 8 chip dies: the die's share of the numbers 0 .. n - 1 is a run of neighbours.
+__device__ __forceinline__ int orth_die_order(int b, int n) {
+  const int x = b & 7, q = n >> 3, r = n & 7;
+  return x * q + min(x, r) + (b >> 3);
 }
 
 __device__ __forceinline__ void split(float v, half_t& hi, half_t& lo) {
@@ -376,7 +389,7 @@ __device__ __forceinline__ void orth_mirror(const OrthArgs& g, const OrthItem& o
 // their way in registers, their four steps of 32 shared out over four groups of four waves, which add their sums through LDS.  (Measured and not kept:
 // fragments straight from memory, no LDS along K, 1.4 to 2 times slower; four waves with the whole tile and a step each, 3 - 8 % slower.)
 template <int TERMS, int KIND, int TILE, int KG, typename OUT>
-__global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin, int last) {
+__global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(OrthArgs g, OUT fin, int last) {
   constexpr int NT = 256 * KG;
     constexpr int KS = TILE == 128 ? (TERMS == 3 ? 32 : 64) : KG == 4 ? 128 : 64;        // K per stage
   constexpr int STAGES = TILE == 128 ? 2 : 1;
@@ -390,11 +403,19 @@ __global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin
   __shared__ __attribute__((aligned(16))) char lds[STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS];
   int t = blockIdx.x, part = 0;
   const bool split_k = TILE == 128 && t >= g.whole;
-  if (split_k) { const int v = t - g.whole; part = v % g.parts; t = g.whole + v / g.parts; }
+  if (TILE == 128 && KIND != kApply) {
+    // a die's workgroups: the same share of K of all tiles (parts in eighths), else neighbouring tiles
+    if (split_k && !(g.parts & 7)) { const int v = t - g.whole; part = v % g.parts; t = g.whole + v / g.parts; }
+    else if (split_k) {
+      const int n = ((int)gridDim.x - g.whole) / g.parts, v = t - g.whole;
+      part = v / n;
+      t = g.whole + orth_die_order(v - part * n, n);
+    } else t = orth_die_order(t, min(g.whole, (int)gridDim.x));
+  }
   int tile, ti, tj; int4 entry;
   const OrthItem o = orth_item(g, t, tile, entry);
   const OrthWs w(o.Mp, o.Np);
-  orth_place(KIND != kApply, tile, entry, o.Np / TILE, ti, tj);
+  orth_place(KIND != kApply, tile, entry, o.Mp / TILE, o.Np / TILE, ti, tj);
   const int tid = threadIdx.x, lane = tid & 63, wid = (tid >> 6) & 3, group = tid >> 8;
   const int wp = (wid & 1) * SIDE, wq = (wid >> 1) * SIDE;              // this wave's part of the tile: entries j, rows i
   char* base = g.ws + o.ws;
@@ -536,7 +557,7 @@ __global__ __launch_bounds__(256 * KG) void orth_gemm_kernel(OrthArgs g, OUT fin
   }
 
   if (split_k) {
-    f32x4* s = g.slab + (long long)(blockIdx.x - g.whole) * (NF * NF * 256);
+    f32x4* s = g.slab + (long long)((t - g.whole) * g.parts + part) * (NF * NF * 256);
 #pragma unroll
     for (int p = 0; p < NF; ++p)
 #pragma unroll
@@ -616,7 +637,7 @@ __global__ __launch_bounds__(256) void orth_join_kernel(OrthArgs g, OUT fin, int
   int tile, ti, tj; int4 entry;
   const OrthItem o = orth_item(g, g.whole + t, tile, entry);
   const OrthWs w(o.Mp, o.Np);
-  orth_place(KIND != kApply, tile, entry, o.Np / 128, ti, tj);
+  orth_place(KIND != kApply, tile, entry, o.Mp / 128, o.Np / 128, ti, tj);
   const int i = ti * 128 + (wid >> 1) * 64 + 16 * q + (lane & 15), j = tj * 128 + (wid & 1) * 64 + 16 * (lane >> 4);
   const OrthPair<16> beside = orth_beside<KIND, 16>(g, o, w, i, j);
   const f32x4* s = g.slab + (long long)t * g.parts * 4096 + q * 256 + tid;
@@ -895,10 +916,12 @@ struct OrthCounts { long long n[4]; int gram_k, poly_k; };       // workgroups o
 
 // How the tiles of a symmetric product share out over 512 places (two workgroups of 128 x 128 tiles per CU): a launch, or its last round, that fills at
 // most three quarters of them is split along K, into parts of 256 at least.  4096 x 4096, 528 tiles: 16 of them alone cost a round as long as the first.
+// (Dealing the stages out evenly instead was slower, 198 against 160 us for 2048 x 8192: workgroups that start at different k share no rows in the L2s.)
 struct OrthSplit { int whole, parts; };
 static OrthSplit orth_split(long long tiles, int K) {
   const long long rest = tiles % 512;
-  const long long parts = rest ? std::min<long long>(512 / rest, K / 256) : 1;
+  long long parts = rest ? std::min<long long>(512 / rest, K / 256) : 1;
+  if (parts > 8) parts &= ~7ll;                          // (in eighths: a chip die's workgroups then share a part's rows in its L2)
   if (rest == 0 || rest > 384 || parts < 2) return {(int)tiles, 1};
   return {(int)(tiles - rest), (int)parts};
 }

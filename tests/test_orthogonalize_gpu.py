@@ -71,6 +71,23 @@ def test_batches(batch, rows, cols, dtype):
     check(np.stack([matrix(rows, cols, "gradient", k) for k in range(batch)]), dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,rows,cols", [(1, 1100, 4400), (4, 500, 2100), (30, 400, 450), (52, 390, 400)])
+def test_products_split_along_k(batch, rows, cols, dtype):
+    """Symmetric products whose tiles do not fill the chip: few of them, a last round of few."""
+    x = np.random.default_rng(5).standard_normal((batch, rows, cols)).astype(np.float32)
+    x[batch // 2:] = x[:batch - batch // 2]                   # (float64 checks two of them; the others have to be the same bits)
+    from pixelwiseregression_amd import ops
+    xt = torch.from_numpy(x).to(dtype)
+    got = ops.orthogonalize(xt.to(DEV)).cpu()
+    for k in {0, (batch - 1) // 2}:
+        ref, tol = bound(xt[k].double().numpy(), dtype == torch.bfloat16)
+        assert np.linalg.norm(got[k].double().numpy() - ref) <= tol
+    one = torch.stack([ops.orthogonalize(xt[k:k + 1].to(DEV))[0].cpu() for k in (0, batch - 1)])
+    for a, b in zip(one, (got[0], got[-1])):                  # (alone, a matrix's sums are split elsewhere: the same up to their rounding)
+        assert (a.double() - b.double()).norm() <= tol
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 6])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_steps_and_coefficients(steps, dtype):
@@ -212,7 +229,7 @@ def test_muon_step(kw):
     muon_case(MIXED, **kw)
 
 
-@pytest.mark.parametrize("shapes", [[(40, 50)], [(7,)], [(1, 1)], [(3000, 2)], [(128, 128, 3, 3)] * 30 + [(128,)] * 30, [(9,), (0,), (4, 0), (4, 4)],
+@pytest.mark.parametrize("shapes", [[(40, 50)], [(7,)], [(1, 1)], [(3000, 2)], [(128, 128, 3, 3)] * 30 + [(128,)] * 30, [(9,), (0,), (4, 0), (4, 4)], [(400, 1200), (500, 2000), (64, 64), (30,), (1000, 1000), (390, 4000)],
                                     [(300, 500), (20000,)]])
 def test_muon_lists(shapes):
     muon_case(shapes, seed=4)
