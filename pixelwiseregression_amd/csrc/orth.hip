@@ -42,7 +42,7 @@ struct OrthItem {
   int rows, cols;           // as the caller has it
   int Mp, Np;               // min / max of the two, up to the tile
   float gain;               // of the update
-  int pad;
+  int shares;               // workgroups along K of a 64 x 64 tile of A
 };
 
 // Its workspace block: X in two buffers (a step reads one and writes the other), A, B, the two diagonals, the partial sums of squares.
@@ -56,13 +56,15 @@ struct OrthWs {
   __host__ __device__ long long parts(int Mp) const { return diag(Mp) + 8ll * Mp; }
 };
 struct OrthArgs {
-  const OrthItem* items; const int4* tiles;              // table form (items != null): tiles[t] = {item, ti, tj, -}
+  const OrthItem* items; const int4* tiles;              // table form (items != null): tiles[t] = {item, ti, tj, share}
   OrthItem one; long long src_stride, dst_stride, ws_stride; int per;     // batch form: t = batch * per + tile
   char* ws;
   int buf;                                               // which X buffer is read
   float a, b, c, eps;
   // a product's tiles from `whole` on are split into `parts` along K: their sums go to slab [tile - whole][part][4 x 4 fragments][256 threads]
   int whole, parts; f32x4* slab;
+  // 64 x 64 tiles: the first `shared` workgroups of A's launch have only a share of their tile's K, and leave their sums at slab + 1024 number
+  int shared;
 };
 
 // the matrix and tile number t of a launch belong to: tile >= 0 is the number within the matrix, else `entry` names it
@@ -412,8 +414,11 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
       t = g.whole + orth_die_order(v - part * n, n);
     } else t = orth_die_order(t, min(g.whole, (int)gridDim.x));
   }
+  constexpr bool SHARED = TILE == 64 && KIND == kGram;
+  if (SHARED && !g.items) { part = t % g.one.shares; t /= g.one.shares; }
   int tile, ti, tj; int4 entry;
   const OrthItem o = orth_item(g, t, tile, entry);
+  if (SHARED && g.items) part = entry.w;
   const OrthWs w(o.Mp, o.Np);
   orth_place(KIND != kApply, tile, entry, o.Mp / TILE, o.Np / TILE, ti, tj);
   const int tid = threadIdx.x, lane = tid & 63, wid = (tid >> 6) & 3, group = tid >> 8;
@@ -522,6 +527,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
   OrthPair<4 * NP> beside[ROWS];
   int kb = 0, ke = K;
   if (split_k) { const int n = K / KS; kb = n * part / g.parts * KS; ke = n * (part + 1) / g.parts * KS; }
+  if (SHARED) { const int n = (K + KS - 1) / KS; kb = n * part / o.shares * KS; ke = min(K, n * (part + 1) / o.shares * KS); }
   const int i0 = ti * TILE + wq + 16 * q0 + li, j0 = tj * TILE + wp + 4 * NF * lg + 4 * p0;
   if constexpr (STAGES == 2) {
     if (kb < ke) { load(kb, 0); store(0, 0); }
@@ -537,22 +543,22 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
       stage ^= 1;
     }
   } else {
-    load(0, 0);
-    if (SETS == 2 && KS < K) load(KS, SETS - 1);
+    load(kb, 0);
+    if (SETS == 2 && kb + KS < ke) load(kb + KS, SETS - 1);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) beside[r] = orth_beside<KIND, 4 * NP>(g, o, w, i0 + 16 * r, j0);
     auto turn = [&](int k0, int set) {
-      if (k0) __syncthreads();                                          // (everyone has read the stage before)
+      if (k0 > kb) __syncthreads();                                          // (everyone has read the stage before)
       store(0, set);
       __syncthreads();
-      if (k0 + SETS * KS < K) load(k0 + SETS * KS, set);
+      if (k0 + SETS * KS < ke) load(k0 + SETS * KS, set);
 #pragma unroll
       for (int kk = 0; kk < KS / 32 / KG; ++kk)
-        if (k0 + (group * (KS / 32 / KG) + kk) * 32 < K) compute(lds, group * (KS / 32 / KG) + kk);
+        if (k0 + (group * (KS / 32 / KG) + kk) * 32 < ke) compute(lds, group * (KS / 32 / KG) + kk);
     };
-    for (int k0 = 0; k0 < K; k0 += SETS * KS) {
+    for (int k0 = kb; k0 < ke; k0 += SETS * KS) {
       turn(k0, 0);
-      if (SETS == 2 && k0 + KS < K) turn(k0 + KS, SETS - 1);
+      if (SETS == 2 && k0 + KS < ke) turn(k0 + KS, SETS - 1);
     }
   }
 
@@ -587,6 +593,10 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
         a = sums[f * KG * 256 + wid * 64 + lane];
 #pragma unroll
         for (int u = 1; u < KG; ++u) a += sums[(f * KG + u) * 256 + wid * 64 + lane];
+      }
+      if constexpr (SHARED) {
+        static_assert(NP == 1 && ROWS == 1, "a thread has one fragment");
+        if (o.shares > 1) { g.slab[(long long)blockIdx.x * 1024 + tid] = a; return; }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[4 * k + e] = a[e];
@@ -631,6 +641,24 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
 }
 
 // the split tiles of a product: a workgroup adds the parts of one of a tile's four fragment rows and finishes it
+// the shared 64 x 64 tiles of A: the workgroup of a tile's first share adds all of them
+template <int TERMS>
+__global__ __launch_bounds__(1024) void orth_join_shared_kernel(OrthArgs g) {
+  const int number = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = (tid >> 6) & 3, group = tid >> 8;
+  int tile, ti, tj; int4 entry;
+  const OrthItem o = orth_item(g, g.items ? number : number / g.one.shares, tile, entry);
+  if ((g.items ? entry.w : number % g.one.shares) != 0) return;
+  const OrthWs w(o.Mp, o.Np);
+  orth_place(true, tile, entry, o.Mp / 64, o.Np / 64, ti, tj);
+  const f32x4* s = g.slab + (long long)number * 1024 + tid;
+  f32x4 a = s[0];
+  for (int u = 1; u < o.shares; ++u) a += s[u * 1024];
+  const int i = ti * 64 + (wid >> 1) * 32 + 16 * (group >> 1) + (lane & 15), j = tj * 64 + (wid & 1) * 32 + 8 * (lane >> 4) + 4 * (group & 1);
+  const float v[4] = {a[0], a[1], a[2], a[3]};
+  const OrthPair<4> d = orth_finish<TERMS, kGram, 4, OrthNone>(g, o, w, OrthNone{}, 0, i, j, v, orth_beside<kGram, 4>(g, o, w, i, j));
+  if (ti != tj) orth_mirror<kGram, 4>(g, o, w, i, j, d);
+}
+
 template <int TERMS, int KIND, typename OUT>
 __global__ __launch_bounds__(256) void orth_join_kernel(OrthArgs g, OUT fin, int last) {
   const int t = blockIdx.x >> 2, q = blockIdx.x & 3, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
@@ -655,7 +683,8 @@ __global__ __launch_bounds__(256) void orth_join_kernel(OrthArgs g, OUT fin, int
 }
 
 // ---- small matrices: one workgroup of eight waves does a whole matrix, X in LDS for all steps.  MT x 16 rows (m <= 32 or 64), up to NCAP columns.
-// Every product is the three-product form, for bf16 tensors too: what is left is latency, not arithmetic.
+// Every product is all four products of the halves, for bf16 tensors too: what is left is latency, not arithmetic, and a sum this short loses less than
+// lo lo: 16 x 40 and 30 x 800 have 0.75 of the error without it, 1 x 7 a seventh, in the same time.
 //   A: a wave pair per quarter of K, each wave half of the 16 x 16 tiles on and above the diagonal; the quarters are added through LDS.
 //   B + a I: two tiles a wave, written over A.      X: a wave takes 16 columns at a time, (B + a I) in registers, and writes them in place.
 template <int MT> struct OrthTri;                       // the tiles (p, q), p <= q, of the two waves of a pair
@@ -725,7 +754,8 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
   });
   __syncthreads();
 
-  auto mfma3 = [](const half8 (&p)[2], const half8 (&q)[2], f32x4 acc) {
+  auto mfma4 = [](const half8 (&p)[2], const half8 (&q)[2], f32x4 acc) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[1], q[1], acc, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[1], q[0], acc, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[0], q[1], acc, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(p[0], q[0], acc, 0, 0, 0);
@@ -749,7 +779,7 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
 #pragma unroll
         for (int p = 0; p < 2; ++p) f[r][p] = *reinterpret_cast<const half8*>(X + p * xplane + xat(16 * r + li, ks * 4 + lg));
 #pragma unroll
-      for (int k = 0; k < NT; ++k) acc[k] = mfma3(f[Tri::p[H][k]], f[Tri::q[H][k]], acc[k]);
+      for (int k = 0; k < NT; ++k) acc[k] = mfma4(f[Tri::p[H][k]], f[Tri::q[H][k]], acc[k]);
     }
     if (quarter) {
 #pragma unroll
@@ -805,7 +835,7 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
           for (int k = 0; k < PW; ++k) fp[k][p] = *reinterpret_cast<const half8*>(R + p * aplane + aat(16 * (p0 + k) + li, kk * 4 + lg));
         }
 #pragma unroll
-        for (int k = 0; k < PW; ++k) acc[k] = mfma3(fp[k], fq, acc[k]);
+        for (int k = 0; k < PW; ++k) acc[k] = mfma4(fp[k], fq, acc[k]);
       }
 #pragma unroll
       for (int k = 0; k < PW; ++k) {
@@ -851,7 +881,7 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
           for (int e = 0; e < 4; ++e) { f[p][e] = lo[e]; f[p][4 + e] = hi[e]; }
         }
 #pragma unroll
-        for (int r = 0; r < MT; ++r) acc[r] = mfma3(f, b[kk][r], acc[r]);
+        for (int r = 0; r < MT; ++r) acc[r] = mfma4(f, b[kk][r], acc[r]);
       }
 #pragma unroll
       for (int r = 0; r < MT; ++r) {
@@ -893,6 +923,7 @@ static OrthItem orth_make(int rows, int cols, int tile) {
   o.rows = rows; o.cols = cols;
   o.Mp = up(std::min(rows, cols), tile); o.Np = up(std::max(rows, cols), tile);
   o.gain = 1.f;
+  o.shares = 1;
   return o;
 }
 // tiles of A or A A (symmetric), and of B X
@@ -912,7 +943,17 @@ static bool orth_is_small(int rows, int cols) {
   return m <= 32 ? n <= 1024 : m <= 64 && n <= 512;
 }
 
-struct OrthCounts { long long n[4]; int gram_k, poly_k; };       // workgroups of the norm, pack, symmetric and B X launches; K of the symmetric ones
+struct OrthCounts { long long n[5]; int gram_k, poly_k; };       // workgroups of the norm, pack, A A, B X and A launches; K of the symmetric ones
+
+// 64 x 64 tiles of A: a workgroup has no more of K than a CU on average (`mean`), but 512 at least, and the rest of its tile is other workgroups', where
+// that shortens the launch by ten stages of 128: what the sums' own launch takes.  fp32, unshared / shared: 20 x 8000 342 / 132 us, 200 x 8000 461 / 193,
+// 4 of 300 x 2000 243 / 201, 13 of 128 x 3200 289 / 220; 13 of 128 x 1152 would be 2 % slower in shares of 384.  (More than 32 shares take one workgroup
+// too long to add; the last workgroup to arrive adding them, without a launch, cost up to 170 us: every one has to write back and drop its L2 first.)
+static int orth_shares(int K, double mean) {
+  const int shares = std::max(1, std::min(32, (int)(K / std::max(512.0, mean) + 0.5)));
+  return K - K / shares >= 1280 ? shares : 1;
+}
+static int orth_shares(const OrthItem& o, int tile, long long tiles) { return tile == 64 ? orth_shares(o.Np, tiles * (double)o.Np / 256) : 1; }
 
 // How the tiles of a symmetric product share out over 512 places (two workgroups of 128 x 128 tiles per CU): a launch, or its last round, that fills at
 // most three quarters of them is split along K, into parts of 256 at least.  4096 x 4096, 528 tiles: 16 of them alone cost a round as long as the first.
@@ -934,9 +975,8 @@ static long long orth_slab_bytes(long long tiles, int gram_k, int poly_k) {
   return most;
 }
 
-// g.slab: behind the matrices' workspaces
 template <int TERMS, int TILE, typename SRC, typename OUT>
-static int orth_run(const OrthArgs& g, const OrthCounts& n, const int4* const (&lists)[4], const SRC& src, const OUT& out, int steps, const int (&per)[4],
+static int orth_run(const OrthArgs& g, const OrthCounts& n, const int4* const (&lists)[5], const SRC& src, const OUT& out, int steps, const int (&per)[5],
                     hipStream_t s) {
   const dim3 b(256);
   constexpr int KG = TILE == 64 ? 4 : 1;
@@ -945,14 +985,18 @@ static int orth_run(const OrthArgs& g, const OrthCounts& n, const int4* const (&
   hipLaunchKernelGGL((orth_pack_kernel<SRC>), dim3((unsigned)n.n[1]), b, 0, s, with(1, 0), src);
   auto symmetric = [&](auto kind, int K, int buf) {
     constexpr int KIND = decltype(kind)::value;
-    OrthArgs h = with(2, buf);
-    long long blocks = n.n[2];
+    constexpr int LIST = KIND == kGram ? 4 : 2;
+    OrthArgs h = with(LIST, buf);
+    long long blocks = n.n[LIST];
     if constexpr (TILE == 128) {
       const OrthSplit sp = orth_split(n.n[2], K);
       h.whole = sp.whole; h.parts = sp.parts;
       blocks = sp.whole + (n.n[2] - sp.whole) * sp.parts;
     }
     hipLaunchKernelGGL((orth_gemm_kernel<TERMS, KIND, TILE, KG, OrthNone>), dim3((unsigned)blocks), dim3(256 * KG), 0, s, h, OrthNone{}, 0);
+    if constexpr (TILE == 64 && KIND == kGram) {
+      if (h.shared) hipLaunchKernelGGL((orth_join_shared_kernel<TERMS>), dim3((unsigned)h.shared), dim3(1024), 0, s, h);
+    }
     if constexpr (TILE == 128) {
       if (h.whole < n.n[2])
         hipLaunchKernelGGL((orth_join_kernel<TERMS, KIND, OrthNone>), dim3((unsigned)(4 * (n.n[2] - h.whole))), b, 0, s, h, OrthNone{}, 0);
@@ -983,7 +1027,8 @@ extern "C" size_t pwr_orthogonalize_workspace_bytes(int rows, int cols, long lon
   if (orth_is_small(rows, cols)) return 256;
   const int tile = orth_tile(rows, cols, batch);
   const OrthItem o = orth_make(rows, cols, tile);
-  return (size_t)(batch * orth_ws_bytes(rows, cols, o.Mp, o.Np) + (tile == 128 ? orth_slab_bytes(batch * orth_sym_tiles(o, 128), o.Np, o.Mp) : 0));
+  const long long tiles = batch * orth_sym_tiles(o, tile), shares = orth_shares(o, tile, tiles);
+  return (size_t)(batch * orth_ws_bytes(rows, cols, o.Mp, o.Np) + (tile == 128 ? orth_slab_bytes(tiles, o.Np, o.Mp) : shares > 1 ? tiles * shares * 16384 : 0));
 }
 
 template <typename T, int TERMS>
@@ -995,13 +1040,16 @@ static int orthogonalize(const void* x, long long x_batch, long long x_ld, void*
   g.ws = (char*)ws;
   g.ws_stride = orth_ws_bytes(rows, cols, g.one.Mp, g.one.Np);
   g.a = a; g.b = b; g.c = c; g.eps = eps;
-  const long long per[4] = {orth_parts(rows, cols), (long long)(g.one.Mp / 64) * (g.one.Np / 64), orth_sym_tiles(g.one, tile), orth_apply_tiles(g.one, tile)};
-  const OrthCounts n = {{batch * per[0], batch * per[1], batch * per[2], batch * per[3]}, g.one.Np, g.one.Mp};
+  const long long sym = orth_sym_tiles(g.one, tile);
+  const long long per[5] = {orth_parts(rows, cols), (long long)(g.one.Mp / 64) * (g.one.Np / 64), sym, orth_apply_tiles(g.one, tile), sym};
+  const int shares = g.one.shares = orth_shares(g.one, tile, batch * sym);
+  const OrthCounts n = {{batch * per[0], batch * per[1], batch * sym, batch * per[3], batch * sym * shares}, g.one.Np, g.one.Mp};
   for (const long long k : n.n)
     if (k > 0x7fffffffll) return PWR_EUNSUPPORTED;
+  g.shared = shares > 1 ? (int)n.n[4] : 0;
   g.slab = (f32x4*)(g.ws + batch * g.ws_stride);
-  const int4* const lists[4] = {};
-  const int iper[4] = {(int)per[0], (int)per[1], (int)per[2], (int)per[3]};
+  const int4* const lists[5] = {};
+  const int iper[5] = {(int)per[0], (int)per[1], (int)per[2], (int)per[3], (int)per[4]};
   g.src_stride = x_batch;
   g.dst_stride = (long long)rows * cols;
   const OrthTensor<T> src = {(const T*)x, x_ld};
@@ -1040,11 +1088,11 @@ namespace {
 constexpr int kRestRun = 4096;           // elements per workgroup of the AdamW part
 struct MuonHead {
   unsigned long long magic, bytes, ws_bytes, slab;
-  int items, tile, gram_k, poly_k;
-  long long n[4], rest;                  // workgroups of the norm, pack, symmetric and apply launches; of the rest
-  long long at_items, at_list[4], at_rest;
+  int items, tile, gram_k, poly_k, shared, pad;
+  long long n[5], rest;                  // workgroups of the norm, pack, A A, B X and A launches; of the rest
+  long long at_items, at_list[5], at_rest;
 };
-constexpr unsigned long long kMuonMagic = 0x31304e4f554d5750ull;
+constexpr unsigned long long kMuonMagic = 0x32304e4f554d5750ull;
 
 // a list is worked on in the tile that most of its products want (in units of a 64 x 64 x 64 block): the rule of orth_tile
 int muon_tile(const std::vector<OrthItem>& v) {
@@ -1083,9 +1131,14 @@ bool muon_layout(const pwr_muon_param* params, int n, MuonHead& h, std::vector<O
   h.items = (int)items.size();
   h.tile = muon_tile(items);
   long long ws = 0;
+  double k_sum = 0;
   for (OrthItem& o : items) {
     const OrthItem q = orth_make(o.rows, o.cols, h.tile);
     o.Mp = q.Mp; o.Np = q.Np;
+    k_sum += orth_sym_tiles(o, h.tile) * (double)o.Np;
+  }
+  for (OrthItem& o : items) {
+    o.shares = h.tile == 64 ? orth_shares(o.Np, k_sum / 256) : 1;
     o.gain = sqrtf((float)std::max(o.rows, o.cols));
     o.ws = ws;
     ws += orth_ws_bytes(o.rows, o.cols, o.Mp, o.Np);
@@ -1093,19 +1146,21 @@ bool muon_layout(const pwr_muon_param* params, int n, MuonHead& h, std::vector<O
     h.n[1] += (long long)(o.Mp / 64) * (o.Np / 64);
     h.n[2] += orth_sym_tiles(o, h.tile);
     h.n[3] += orth_apply_tiles(o, h.tile);
+    h.n[4] += orth_sym_tiles(o, h.tile) * o.shares;
+    if (o.shares > 1) h.shared += (int)(orth_sym_tiles(o, h.tile) * o.shares);
     h.gram_k = std::max(h.gram_k, o.Np);
     h.poly_k = std::max(h.poly_k, o.Mp);
   }
   h.slab = ws;
-  h.ws_bytes = ws + (h.tile == 128 ? orth_slab_bytes(h.n[2], h.gram_k, h.poly_k) : 0);
+  h.ws_bytes = ws + (h.tile == 128 ? orth_slab_bytes(h.n[2], h.gram_k, h.poly_k) : h.shared * 16384ll);
   h.rest = (long long)rest.size();
   long long at = (sizeof(MuonHead) + 255) / 256 * 256;
   auto take = [&](long long bytes) { const long long r = at; at += (bytes + 255) / 256 * 256; return r; };
   h.at_items = take(h.items * (long long)sizeof(OrthItem));
-  for (int k = 0; k < 4; ++k) h.at_list[k] = take(h.n[k] * (long long)sizeof(int4));
+  for (int k = 0; k < 5; ++k) h.at_list[k] = take(h.n[k] * (long long)sizeof(int4));
   h.at_rest = take(h.rest * (long long)sizeof(longlong2));
   h.bytes = at;
-  for (int k = 0; k < 4; ++k)
+  for (int k = 0; k < 5; ++k)
     if (h.n[k] > 0x7fffffffll) return false;
   return h.rest <= 0x7fffffffll;
 }
@@ -1130,18 +1185,32 @@ extern "C" int pwr_muon_plan(const pwr_muon_param* params, int n, void* host_dst
   memset(d, 0, h.bytes);
   memcpy(d, &h, sizeof h);
   memcpy(d + h.at_items, items.data(), items.size() * sizeof(OrthItem));
-  std::vector<int4> list[4];
+  // The longest sums first (of A: the longest rows; of A A and B X: the most rows), so that a launch does not end on them; of A that puts the shared tiles in front.
+  std::vector<int> by_k(h.items), by_m(h.items);
+  for (int k = 0; k < h.items; ++k) by_k[k] = by_m[k] = k;
+  std::stable_sort(by_k.begin(), by_k.end(), [&](int p, int q) { return items[p].Np > items[q].Np; });
+  std::stable_sort(by_m.begin(), by_m.end(), [&](int p, int q) { return items[p].Mp > items[q].Mp; });
+  std::vector<int4> list[5];
   for (int k = 0; k < h.items; ++k) {
     const OrthItem& o = items[k];
     for (int t = 0; t < orth_parts(o.rows, o.cols); ++t) list[0].push_back(int4{k, t, 0, 0});
     for (int i = 0; i < o.Mp / 64; ++i)
       for (int j = 0; j < o.Np / 64; ++j) list[1].push_back(int4{k, i, j, 0});
+  }
+  for (const int k : by_m) {
+    const OrthItem& o = items[k];
     for (int j = 0; j < o.Mp / h.tile; ++j)
       for (int i = 0; i <= j; ++i) list[2].push_back(int4{k, i, j, 0});
     for (int i = 0; i < o.Mp / h.tile; ++i)
       for (int j = 0; j < o.Np / h.tile; ++j) list[3].push_back(int4{k, i, j, 0});
   }
-  for (int k = 0; k < 4; ++k) memcpy(d + h.at_list[k], list[k].data(), list[k].size() * sizeof(int4));
+  for (const int k : by_k) {
+    const OrthItem& o = items[k];
+    for (int j = 0; j < o.Mp / h.tile; ++j)
+      for (int i = 0; i <= j; ++i)
+        for (int u = 0; u < o.shares; ++u) list[4].push_back(int4{k, i, j, u});
+  }
+  for (int k = 0; k < 5; ++k) memcpy(d + h.at_list[k], list[k].data(), list[k].size() * sizeof(int4));
   memcpy(d + h.at_rest, rest.data(), rest.size() * sizeof(longlong2));
   return 0;
 }
@@ -1172,12 +1241,13 @@ extern "C" int pwr_muon_step(const void* plan_host, const void* plan_dev, float*
   ga.items = (const OrthItem*)(d + h->at_items);
   ga.ws = (char*)workspace;
   ga.a = a; ga.b = b; ga.c = c; ga.eps = eps;
-  const OrthCounts n = {{h->n[0], h->n[1], h->n[2], h->n[3]}, h->gram_k, h->poly_k};
+  const OrthCounts n = {{h->n[0], h->n[1], h->n[2], h->n[3], h->n[4]}, h->gram_k, h->poly_k};
+  ga.shared = h->shared;
   ga.slab = (f32x4*)(ga.ws + h->slab);
-  const int4* lists[4];
-  for (int k = 0; k < 4; ++k) lists[k] = (const int4*)(d + h->at_list[k]);
-  const int4* const (&ls)[4] = lists;
-  const int per[4] = {};
+  const int4* lists[5];
+  for (int k = 0; k < 5; ++k) lists[k] = (const int4*)(d + h->at_list[k]);
+  const int4* const (&ls)[5] = lists;
+  const int per[5] = {};
   const OrthMomentum src = {g, buf, momentum, grad_scale, nesterov};
   const OrthUpdate dst = {p, keep, lr * update_rms};
   return h->tile == 128 ? orth_run<3, 128>(ga, n, ls, src, dst, ns_steps, per, s) : orth_run<3, 64>(ga, n, ls, src, dst, ns_steps, per, s);

@@ -72,9 +72,10 @@ def test_batches(batch, rows, cols, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("batch,rows,cols", [(1, 1100, 4400), (4, 500, 2100), (30, 400, 450), (52, 390, 400)])
+@pytest.mark.parametrize("batch,rows,cols", [(1, 1100, 4400), (4, 500, 2100), (30, 400, 450), (52, 390, 400), (1, 20, 8000), (3, 2300, 70), (4, 300, 2000),
+                                             (2, 6, 70000)])
 def test_products_split_along_k(batch, rows, cols, dtype):
-    """Symmetric products whose tiles do not fill the chip: few of them, a last round of few."""
+    """Symmetric products whose tiles do not fill the chip: few of them, a last round of few, small ones with long sums."""
     x = np.random.default_rng(5).standard_normal((batch, rows, cols)).astype(np.float32)
     x[batch // 2:] = x[:batch - batch // 2]                   # (float64 checks two of them; the others have to be the same bits)
     from pixelwiseregression_amd import ops
@@ -230,7 +231,7 @@ def test_muon_step(kw):
 
 
 @pytest.mark.parametrize("shapes", [[(40, 50)], [(7,)], [(1, 1)], [(3000, 2)], [(128, 128, 3, 3)] * 30 + [(128,)] * 30, [(9,), (0,), (4, 0), (4, 4)], [(400, 1200), (500, 2000), (64, 64), (30,), (1000, 1000), (390, 4000)],
-                                    [(300, 500), (20000,)]])
+                                    [(300, 500), (20000,)], [(64, 64), (20, 8000), (9,), (128, 3200), (2100, 60), (3, 100)]])
 def test_muon_lists(shapes):
     muon_case(shapes, seed=4)
 
