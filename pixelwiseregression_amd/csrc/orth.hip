@@ -82,11 +82,18 @@ __device__ __forceinline__ OrthItem orth_item(const OrthArgs& g, int t, int& til
   o.ws += batch * g.ws_stride;
   return o;
 }
+// Tiles of B X: a die gets every eighth workgroup.  64 x 64 tiles go in bands of eight columns, so that a die has a column of X for all its rows (5 of
+// 1031 x 517 fp32 300 -> 265 us, the step of the 42-joint network with 256 features 530 -> 515); 128 x 128 ones row by row: eight columns and eight rows at once on a die (2048 x 8192 2010 us, in bands 2060).
+__host__ __device__ __forceinline__ int orth_band(int tile, int nj) { return tile == 64 ? 8 : nj; }
 // (ti, tj) of a tile of B X, or of a symmetric product: ti <= tj, in blocks of 4 x 4 tiles, block column J from tile 2 J (4 J + 1) on: workgroups that run
-// together on a chip die read few different rows.  T: tiles a side; nj: tiles a row of X.
-__device__ __forceinline__ void orth_place(bool symmetric, int tile, const int4& entry, int T, int nj, int& ti, int& tj) {
+// together on a chip die read few different rows.  T: tiles a side; nj: tiles a row of X, `band` of them at a time.
+__device__ __forceinline__ void orth_place(bool symmetric, int tile, const int4& entry, int T, int nj, int band, int& ti, int& tj) {
   if (tile < 0) { ti = entry.y; tj = entry.z; }
-  else if (!symmetric) { ti = tile / nj; tj = tile - ti * nj; }
+  else if (!symmetric) {
+    const int b = tile / (band * T), rest = tile - b * band * T, wide = min(band, nj - b * band);
+    ti = rest / wide;
+    tj = b * band + rest - ti * wide;
+  }
   else {
     int J = (int)((sqrtf(4.f + 32.f * tile) - 2.f) * (1.f / 16.f));
     while (2 * J * (4 * J + 1) > tile) --J;
@@ -415,12 +422,14 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
     } else t = orth_die_order(t, min(g.whole, (int)gridDim.x));
   }
   constexpr bool SHARED = TILE == 64 && KIND == kGram;
+  // (64 x 64 tiles: neighbours on a die from 16 tiles a die on.  5 of 1031 x 517 fp32 265 -> 247 us; 700 x 1000, 66 tiles, would be 198 -> 206)
+  if (TILE == 64 && KIND != kApply && !g.items && gridDim.x >= 128 && (KIND == kPoly || g.one.shares == 1)) t = orth_die_order(t, gridDim.x);
   if (SHARED && !g.items) { part = t % g.one.shares; t /= g.one.shares; }
   int tile, ti, tj; int4 entry;
   const OrthItem o = orth_item(g, t, tile, entry);
   if (SHARED && g.items) part = entry.w;
   const OrthWs w(o.Mp, o.Np);
-  orth_place(KIND != kApply, tile, entry, o.Mp / TILE, o.Np / TILE, ti, tj);
+  orth_place(KIND != kApply, tile, entry, o.Mp / TILE, o.Np / TILE, orth_band(TILE, o.Np / TILE), ti, tj);
   const int tid = threadIdx.x, lane = tid & 63, wid = (tid >> 6) & 3, group = tid >> 8;
   const int wp = (wid & 1) * SIDE, wq = (wid >> 1) * SIDE;              // this wave's part of the tile: entries j, rows i
   char* base = g.ws + o.ws;
@@ -649,7 +658,7 @@ __global__ __launch_bounds__(1024) void orth_join_shared_kernel(OrthArgs g) {
   const OrthItem o = orth_item(g, g.items ? number : number / g.one.shares, tile, entry);
   if ((g.items ? entry.w : number % g.one.shares) != 0) return;
   const OrthWs w(o.Mp, o.Np);
-  orth_place(true, tile, entry, o.Mp / 64, o.Np / 64, ti, tj);
+  orth_place(true, tile, entry, o.Mp / 64, o.Np / 64, 1, ti, tj);
   const f32x4* s = g.slab + (long long)number * 1024 + tid;
   f32x4 a = s[0];
   for (int u = 1; u < o.shares; ++u) a += s[u * 1024];
@@ -665,7 +674,7 @@ __global__ __launch_bounds__(256) void orth_join_kernel(OrthArgs g, OUT fin, int
   int tile, ti, tj; int4 entry;
   const OrthItem o = orth_item(g, g.whole + t, tile, entry);
   const OrthWs w(o.Mp, o.Np);
-  orth_place(KIND != kApply, tile, entry, o.Mp / 128, o.Np / 128, ti, tj);
+  orth_place(KIND != kApply, tile, entry, o.Mp / 128, o.Np / 128, 1, ti, tj);
   const int i = ti * 128 + (wid >> 1) * 64 + 16 * q + (lane & 15), j = tj * 128 + (wid & 1) * 64 + 16 * (lane >> 4);
   const OrthPair<16> beside = orth_beside<KIND, 16>(g, o, w, i, j);
   const f32x4* s = g.slab + (long long)t * g.parts * 4096 + q * 256 + tid;
@@ -1201,8 +1210,10 @@ extern "C" int pwr_muon_plan(const pwr_muon_param* params, int n, void* host_dst
     const OrthItem& o = items[k];
     for (int j = 0; j < o.Mp / h.tile; ++j)
       for (int i = 0; i <= j; ++i) list[2].push_back(int4{k, i, j, 0});
-    for (int i = 0; i < o.Mp / h.tile; ++i)
-      for (int j = 0; j < o.Np / h.tile; ++j) list[3].push_back(int4{k, i, j, 0});
+    const int nj = o.Np / h.tile, band = orth_band(h.tile, nj);
+    for (int j0 = 0; j0 < nj; j0 += band)
+      for (int i = 0; i < o.Mp / h.tile; ++i)
+        for (int j = j0; j < std::min(nj, j0 + band); ++j) list[3].push_back(int4{k, i, j, 0});
   }
   for (const int k : by_k) {
     const OrthItem& o = items[k];
