@@ -34,6 +34,7 @@ typedef __attribute__((ext_vector_type(4))) _Float16 half4;
 
 constexpr float kOrthScale = 4096.f;                     // of every stored pair
 constexpr float kOrthInv = 1.f / 4096.f;
+constexpr int kOrthNarrow = 128;                         // up to this many rows A fits the LDS: its sums go straight into the product A A
 
 // One matrix.  In a table on the device (a parameter list), or made from the launch's arguments (a batch of equal ones).
 struct OrthItem {
@@ -42,7 +43,7 @@ struct OrthItem {
   int rows, cols;           // as the caller has it
   int Mp, Np;               // min / max of the two, up to the tile
   float gain;               // of the update
-  int shares;               // workgroups along K of a 64 x 64 tile of A
+  int shares, first;        // workgroups along K of a 64 x 64 tile of A; the first workgroup of its tiles (in a batch: workgroups per matrix)
 };
 
 // Its workspace block: X in two buffers (a step reads one and writes the other), A, B, the two diagonals, the partial sums of squares.
@@ -63,7 +64,8 @@ struct OrthArgs {
   float a, b, c, eps;
   // a product's tiles from `whole` on are split into `parts` along K: their sums go to slab [tile - whole][part][4 x 4 fragments][256 threads]
   int whole, parts; f32x4* slab;
-  // 64 x 64 tiles: the first `shared` workgroups of A's launch have only a share of their tile's K, and leave their sums at slab + 1024 number
+  // 64 x 64 tiles: a workgroup of A that has only a share of its tile's K, or whose matrix is narrow, leaves its sums at slab + 1024 number; the first
+  // `shared` ones are joined by a launch of their own
   int shared;
 };
 
@@ -80,6 +82,7 @@ __device__ __forceinline__ OrthItem orth_item(const OrthArgs& g, int t, int& til
   o.src += batch * g.src_stride;
   o.dst += batch * g.dst_stride;
   o.ws += batch * g.ws_stride;
+  o.first *= batch;
   return o;
 }
 // Tiles of B X: a die gets every eighth workgroup.  64 x 64 tiles go in bands of eight columns, so that a die has a column of X for all its rows (5 of
@@ -324,7 +327,7 @@ __device__ __forceinline__ OrthPair<N> orth_beside(const OrthArgs& g, const Orth
 // Entries (i, j .. j + N) of a finished product, and what becomes of them: A, B or the next X, as pairs (returned too); after the last step the result.
 template <int TERMS, int KIND, int N, typename OUT>
 __device__ __forceinline__ OrthPair<N> orth_finish(const OrthArgs& g, const OrthItem& o, const OrthWs& w, const OUT& fin, int last, int i, int j,
-                                                   const float (&sum)[N], const OrthPair<N>& beside) {
+                                                   const float (&sum)[N], const OrthPair<N>& beside, const float* diag = nullptr) {
   char* base = g.ws + o.ws;
   float v[N];
   OrthPair<N> r;
@@ -351,13 +354,14 @@ __device__ __forceinline__ OrthPair<N> orth_finish(const OrthArgs& g, const Orth
     }
   } else {
     if constexpr (KIND == kPoly) {
-      const float di = TERMS == 1 ? dA[i] : 0.f;
+      const float* const da = diag ? diag : dA;
+      const float di = TERMS == 1 ? da[i] : 0.f;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         float aij = ((float)beside.h.v[e] + (float)beside.l.v[e]) * kOrthInv, aa = v[e];
         if constexpr (TERMS == 1) {
           if (i == j + e) { aij = di; aa = fmaf(di, di, aa); }
-          else aa = fmaf(di + dA[j + e], aij, aa);
+          else aa = fmaf(di + da[j + e], aij, aa);
         }
         v[e] = fmaf(g.c, aa, g.b * aij);
       }
@@ -385,6 +389,74 @@ __device__ __forceinline__ void orth_mirror(const OrthArgs& g, const OrthItem& o
     dst[(long long)(j + e) * o.Mp] = r.h.v[e];
     dst[w.aplane + (long long)(j + e) * o.Mp] = r.l.v[e];
   }
+}
+
+// A A of a matrix of one or two 64 x 64 tiles a side: the workgroup (16 waves, a fragment each) adds the shares of all of A into LDS, which is never
+// written out, and multiplies from there.
+template <int TERMS>
+__device__ __forceinline__ void orth_narrow_poly(const OrthArgs& g, const OrthItem& o, const OrthWs& w, int ti, int tj, char* lds) {
+  __shared__ float diag[kOrthNarrow];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
+  const int Mp = o.Mp, plane = Mp * Mp * 2, flip = Mp == 128 ? 15 : 7, shift = Mp == 128 ? 0 : 1;
+  // rows of Mp * 2 bytes, their 16-byte units swizzled by the row
+  auto at = [&](int row, int j) { return row * Mp * 2 + (((j >> 3) ^ ((row >> shift) & flip)) << 4) + (j & 7) * 2; };
+  const f32x4* s = g.slab + (long long)o.first * 1024 + tid;
+  const int gi = ((wave >> 1) & 1) * 32 + (wave >> 3) * 16 + li, gj = (wave & 1) * 32 + 8 * lg + ((wave >> 2) & 1) * 4;     // the entries that A's launch gave this thread
+  auto place = [&](const f32x4& a, int i, int j, bool mirror) {
+    half4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v = a[e] * (kOrthInv * kOrthInv);
+      if (TERMS == 1 && i == j + e) { diag[i] = v; v = 0.f; }
+      half_t p, q;
+      split(v, p, q);
+      h[e] = p; l[e] = q;
+    }
+    *reinterpret_cast<half4*>(lds + at(i, j)) = h;
+    *reinterpret_cast<half4*>(lds + plane + at(i, j)) = l;
+    if (mirror) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        *reinterpret_cast<half_t*>(lds + at(j + e, i)) = h[e];
+        *reinterpret_cast<half_t*>(lds + plane + at(j + e, i)) = l[e];
+      }
+    }
+  };
+  const int n = o.shares;
+  if (Mp == 64) {
+    f32x4 a = s[0];
+    for (int u = 1; u < n; ++u) a += s[u * 1024];
+    place(a, gi, gj, false);
+  } else {
+    f32x4 a[3];
+#pragma unroll
+    for (int q = 0; q < 3; ++q) a[q] = s[q * n * 1024];
+    for (int u = 1; u < n; ++u)
+#pragma unroll
+      for (int q = 0; q < 3; ++q) a[q] += s[(q * n + u) * 1024];
+    place(a[0], gi, gj, false);
+    place(a[1], gi, 64 + gj, true);
+    place(a[2], 64 + gi, 64 + gj, false);
+  }
+  __syncthreads();
+  const int i = ti * 64 + (wave >> 2) * 16, j = tj * 64 + (wave & 3) * 16;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 8 * lg; k < Mp; k += 32) {
+    const half8 qh = *reinterpret_cast<const half8*>(lds + at(i + li, k)), ph = *reinterpret_cast<const half8*>(lds + at(j + li, k));
+    if constexpr (TERMS == 3) {
+      const half8 ql = *reinterpret_cast<const half8*>(lds + plane + at(i + li, k)), pl = *reinterpret_cast<const half8*>(lds + plane + at(j + li, k));
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, acc, 0, 0, 0);
+    }
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
+  }
+  const int jj = j + 4 * lg;
+  OrthPair<4> beside;
+  beside.h = *reinterpret_cast<const Halves<4>*>(lds + at(i + li, jj));
+  beside.l = *reinterpret_cast<const Halves<4>*>(lds + plane + at(i + li, jj));
+  const float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+  const OrthPair<4> d = orth_finish<TERMS, kPoly, 4, OrthNone>(g, o, w, OrthNone{}, 0, i + li, jj, v, beside, diag);
+  if (ti != tj) orth_mirror<kPoly, 4>(g, o, w, i + li, jj, d);
 }
 
 // ---- the products: one TILE x TILE tile of the result per workgroup of four waves.
@@ -431,6 +503,12 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
   const OrthWs w(o.Mp, o.Np);
   orth_place(KIND != kApply, tile, entry, o.Mp / TILE, o.Np / TILE, orth_band(TILE, o.Np / TILE), ti, tj);
   const int tid = threadIdx.x, lane = tid & 63, wid = (tid >> 6) & 3, group = tid >> 8;
+  if constexpr (TILE == 64 && KIND == kPoly) {
+    if (o.Mp <= kOrthNarrow) {
+      orth_narrow_poly<TERMS>(g, o, w, ti, tj, lds);
+      return;
+    }
+  }
   const int wp = (wid & 1) * SIDE, wq = (wid >> 1) * SIDE;              // this wave's part of the tile: entries j, rows i
   char* base = g.ws + o.ws;
   const half_t* X = reinterpret_cast<const half_t*>(base + w.x(g.buf));
@@ -605,7 +683,10 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
       }
       if constexpr (SHARED) {
         static_assert(NP == 1 && ROWS == 1, "a thread has one fragment");
-        if (o.shares > 1) { g.slab[(long long)blockIdx.x * 1024 + tid] = a; return; }
+        if (o.shares > 1 || o.Mp <= kOrthNarrow) {
+          g.slab[(long long)(g.items ? (int)blockIdx.x : t * o.shares + part) * 1024 + tid] = a;
+          return;
+        }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[4 * k + e] = a[e];
@@ -954,15 +1035,14 @@ static bool orth_is_small(int rows, int cols) {
 
 struct OrthCounts { long long n[5]; int gram_k, poly_k; };       // workgroups of the norm, pack, A A, B X and A launches; K of the symmetric ones
 
-// 64 x 64 tiles of A: a workgroup has no more of K than a CU on average (`mean`), but 512 at least, and the rest of its tile is other workgroups', where
-// that shortens the launch by ten stages of 128: what the sums' own launch takes.  fp32, unshared / shared: 20 x 8000 342 / 132 us, 200 x 8000 461 / 193,
-// 4 of 300 x 2000 243 / 201, 13 of 128 x 3200 289 / 220; 13 of 128 x 1152 would be 2 % slower in shares of 384.  (More than 32 shares take one workgroup
-// too long to add; the last workgroup to arrive adding them, without a launch, cost up to 170 us: every one has to write back and drop its L2 first.)
-static int orth_shares(int K, double mean) {
-  const int shares = std::max(1, std::min(32, (int)(K / std::max(512.0, mean) + 0.5)));
-  return K - K / shares >= 1280 ? shares : 1;
+// 64 x 64 tiles of A: a workgroup has no more of K than a CU on average (`mean`), but 512 at least, and the rest of its tile is other workgroups'.  The
+// sums of a narrow matrix go into A A as they are; others need a launch that joins them, which has to save ten stages of 128.  fp32, unshared / shared:
+// 20 x 8000 342 / 117 us, 13 of 128 x 1152 132 / 116, 200 x 8000 461 / 193, 4 of 300 x 2000 243 / 201.  (In shares of 256 the first is 132; more than 32
+// take one workgroup too long to add.  The last workgroup to arrive adding them cost up to 170 us a launch: every one has to write back and drop its L2.)
+static int orth_shares(const OrthItem& o, double mean) {
+  const int shares = std::max(1, std::min(32, (int)(o.Np / std::max(512.0, mean) + 0.5)));
+  return o.Mp <= kOrthNarrow || o.Np - o.Np / shares >= 1280 ? shares : 1;
 }
-static int orth_shares(const OrthItem& o, int tile, long long tiles) { return tile == 64 ? orth_shares(o.Np, tiles * (double)o.Np / 256) : 1; }
 
 // How the tiles of a symmetric product share out over 512 places (two workgroups of 128 x 128 tiles per CU): a launch, or its last round, that fills at
 // most three quarters of them is split along K, into parts of 256 at least.  4096 x 4096, 528 tiles: 16 of them alone cost a round as long as the first.
@@ -1036,8 +1116,9 @@ extern "C" size_t pwr_orthogonalize_workspace_bytes(int rows, int cols, long lon
   if (orth_is_small(rows, cols)) return 256;
   const int tile = orth_tile(rows, cols, batch);
   const OrthItem o = orth_make(rows, cols, tile);
-  const long long tiles = batch * orth_sym_tiles(o, tile), shares = orth_shares(o, tile, tiles);
-  return (size_t)(batch * orth_ws_bytes(rows, cols, o.Mp, o.Np) + (tile == 128 ? orth_slab_bytes(tiles, o.Np, o.Mp) : shares > 1 ? tiles * shares * 16384 : 0));
+  const long long tiles = batch * orth_sym_tiles(o, tile), shares = orth_shares(o, tiles * (double)o.Np / 256);
+  const long long sums = tile == 128 ? orth_slab_bytes(tiles, o.Np, o.Mp) : shares > 1 || o.Mp <= kOrthNarrow ? tiles * shares * 16384 : 0;
+  return (size_t)(batch * orth_ws_bytes(rows, cols, o.Mp, o.Np) + sums);
 }
 
 template <typename T, int TERMS>
@@ -1051,11 +1132,12 @@ static int orthogonalize(const void* x, long long x_batch, long long x_ld, void*
   g.a = a; g.b = b; g.c = c; g.eps = eps;
   const long long sym = orth_sym_tiles(g.one, tile);
   const long long per[5] = {orth_parts(rows, cols), (long long)(g.one.Mp / 64) * (g.one.Np / 64), sym, orth_apply_tiles(g.one, tile), sym};
-  const int shares = g.one.shares = orth_shares(g.one, tile, batch * sym);
+  const int shares = g.one.shares = tile == 64 ? orth_shares(g.one, batch * sym * (double)g.one.Np / 256) : 1;
+  g.one.first = (int)(sym * shares);
   const OrthCounts n = {{batch * per[0], batch * per[1], batch * sym, batch * per[3], batch * sym * shares}, g.one.Np, g.one.Mp};
   for (const long long k : n.n)
     if (k > 0x7fffffffll) return PWR_EUNSUPPORTED;
-  g.shared = shares > 1 ? (int)n.n[4] : 0;
+  g.shared = shares > 1 && g.one.Mp > kOrthNarrow ? (int)n.n[4] : 0;
   g.slab = (f32x4*)(g.ws + batch * g.ws_stride);
   const int4* const lists[5] = {};
   const int iper[5] = {(int)per[0], (int)per[1], (int)per[2], (int)per[3], (int)per[4]};
@@ -1141,13 +1223,14 @@ bool muon_layout(const pwr_muon_param* params, int n, MuonHead& h, std::vector<O
   h.tile = muon_tile(items);
   long long ws = 0;
   double k_sum = 0;
+  bool sums = false;
   for (OrthItem& o : items) {
     const OrthItem q = orth_make(o.rows, o.cols, h.tile);
     o.Mp = q.Mp; o.Np = q.Np;
     k_sum += orth_sym_tiles(o, h.tile) * (double)o.Np;
   }
   for (OrthItem& o : items) {
-    o.shares = h.tile == 64 ? orth_shares(o.Np, k_sum / 256) : 1;
+    o.shares = h.tile == 64 ? orth_shares(o, k_sum / 256) : 1;
     o.gain = sqrtf((float)std::max(o.rows, o.cols));
     o.ws = ws;
     ws += orth_ws_bytes(o.rows, o.cols, o.Mp, o.Np);
@@ -1156,12 +1239,13 @@ bool muon_layout(const pwr_muon_param* params, int n, MuonHead& h, std::vector<O
     h.n[2] += orth_sym_tiles(o, h.tile);
     h.n[3] += orth_apply_tiles(o, h.tile);
     h.n[4] += orth_sym_tiles(o, h.tile) * o.shares;
-    if (o.shares > 1) h.shared += (int)(orth_sym_tiles(o, h.tile) * o.shares);
+    if (o.shares > 1 && o.Mp > kOrthNarrow) h.shared += (int)(orth_sym_tiles(o, h.tile) * o.shares);
+    sums = sums || o.shares > 1 || o.Mp <= kOrthNarrow;
     h.gram_k = std::max(h.gram_k, o.Np);
     h.poly_k = std::max(h.poly_k, o.Mp);
   }
   h.slab = ws;
-  h.ws_bytes = ws + (h.tile == 128 ? orth_slab_bytes(h.n[2], h.gram_k, h.poly_k) : h.shared * 16384ll);
+  h.ws_bytes = ws + (h.tile == 128 ? orth_slab_bytes(h.n[2], h.gram_k, h.poly_k) : sums ? h.n[4] * 16384 : 0);
   h.rest = (long long)rest.size();
   long long at = (sizeof(MuonHead) + 255) / 256 * 256;
   auto take = [&](long long bytes) { const long long r = at; at += (bytes + 255) / 256 * 256; return r; };
@@ -1193,11 +1277,14 @@ extern "C" int pwr_muon_plan(const pwr_muon_param* params, int n, void* host_dst
   char* d = (char*)host_dst;
   memset(d, 0, h.bytes);
   memcpy(d, &h, sizeof h);
-  memcpy(d + h.at_items, items.data(), items.size() * sizeof(OrthItem));
-  // The longest sums first (of A: the longest rows; of A A and B X: the most rows), so that a launch does not end on them; of A that puts the shared tiles in front.
+  // The longest sums first (of A: the longest rows; of A A and B X: the most rows), so that a launch does not end on them; of A the tiles with a
+  // launch that joins them are in front.
   std::vector<int> by_k(h.items), by_m(h.items);
   for (int k = 0; k < h.items; ++k) by_k[k] = by_m[k] = k;
-  std::stable_sort(by_k.begin(), by_k.end(), [&](int p, int q) { return items[p].Np > items[q].Np; });
+  std::stable_sort(by_k.begin(), by_k.end(), [&](int p, int q) {
+    const bool jp = items[p].shares > 1 && items[p].Mp > kOrthNarrow, jq = items[q].shares > 1 && items[q].Mp > kOrthNarrow;
+    return jp != jq ? jp : items[p].Np > items[q].Np;
+  });
   std::stable_sort(by_m.begin(), by_m.end(), [&](int p, int q) { return items[p].Mp > items[q].Mp; });
   std::vector<int4> list[5];
   for (int k = 0; k < h.items; ++k) {
@@ -1216,11 +1303,13 @@ extern "C" int pwr_muon_plan(const pwr_muon_param* params, int n, void* host_dst
         for (int j = j0; j < std::min(nj, j0 + band); ++j) list[3].push_back(int4{k, i, j, 0});
   }
   for (const int k : by_k) {
-    const OrthItem& o = items[k];
+    OrthItem& o = items[k];
+    o.first = (int)list[4].size();
     for (int j = 0; j < o.Mp / h.tile; ++j)
       for (int i = 0; i <= j; ++i)
         for (int u = 0; u < o.shares; ++u) list[4].push_back(int4{k, i, j, u});
   }
+  memcpy(d + h.at_items, items.data(), items.size() * sizeof(OrthItem));
   for (int k = 0; k < 5; ++k) memcpy(d + h.at_list[k], list[k].data(), list[k].size() * sizeof(int4));
   memcpy(d + h.at_rest, rest.data(), rest.size() * sizeof(longlong2));
   return 0;
