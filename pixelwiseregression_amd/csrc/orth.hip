@@ -807,40 +807,66 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
   auto xat = [&](int row, int unit) { return row * NP * 2 + ((unit ^ (odd ? (row >> 1) & 7 : row & 7)) << 4); };
   auto aat = [&](int row, int unit) { return row * MP * 2 + ((unit ^ ((row >> 1) & (MP / 8 - 1))) << 4); };
 
-  // |G|, then X0: the source is read twice, the second time from the caches
+  // |G|, then X0: the source is read once, all of a thread's loads under way together: four neighbours of a row at a time, number tid + 512 k
   for (int k = tid * 16; k < 2 * xplane; k += 512 * 16) *reinterpret_cast<uint4*>(X + k) = uint4{0, 0, 0, 0};
-  const int total = o.rows * o.cols, dr = 512 / o.cols, dc = 512 % o.cols;
+  constexpr int PER = MP * NCAP / 2048, RUN = PER < 4 ? PER : 4;
+  const int wide = (o.cols + 3) >> 2, quads = o.rows * wide, dr = 512 / wide, dc = 512 % wide, r0 = tid / wide;
   const long long ld = src.stride(o);
-  auto sweep = [&](auto&& use) {
-    int r = tid / o.cols, c = tid - r * o.cols;
-    for (int base = tid; base - tid < total; base += 8 * 512) {
-      float v[8];
-      int rr[8], cc[8];
+  float v[PER][4];
+  auto sweep = [&](auto&& use) {                        // (r, c): the row and the first column of the four
+    int r = r0, c = tid - r0 * wide;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        rr[u] = r; cc[u] = c;
-        v[u] = src.one(o, min(r, o.rows - 1) * ld + c);
-        r += dr; c += dc;
-        if (c >= o.cols) { c -= o.cols; ++r; }
+    for (int k0 = 0; k0 < PER; k0 += RUN)
+      if (k0 * 512 < quads) {
+#pragma unroll
+        for (int k = k0; k < k0 + RUN; ++k) {
+          use(v[k], r, 4 * c);
+          r += dr; c += dc;
+          if (c >= wide) { c -= wide; ++r; }
+        }
       }
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (rr[u] < o.rows) use(rr[u], cc[u], v[u]);
-    }
   };
+  if (o.cols & 3) {
+    sweep([&](float (&q)[4], int r, int c) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = src.one(o, min(r, o.rows - 1) * ld + min(c + e, o.cols - 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = r < o.rows && c + e < o.cols ? q[e] : 0.f;
+    });
+  } else {
+    sweep([&](float (&q)[4], int r, int c) {
+      src.quad(o, min(r, o.rows - 1) * ld + c, q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = r < o.rows ? q[e] : 0.f;
+    });
+  }
   double s = 0.0;
-  sweep([&](int, int, float v) { s += (double)v * v; });
+  sweep([&](float (&q)[4], int, int) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += (double)q[e] * q[e];
+  });
   for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
   if (lane == 0) red[wid] = s;
   __syncthreads();
   s = ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
   const double inv = 1.0 / (sqrt(s) + (double)g.eps);
-  sweep([&](int r, int c, float v) {
-    half_t hi, lo;
-    split((float)((double)v * inv), hi, lo);
-    const int i = tall ? c : r, j = tall ? r : c, at = xat(i, j >> 3) + (j & 7) * 2;
-    *reinterpret_cast<half_t*>(X + at) = hi;
-    *reinterpret_cast<half_t*>(X + xplane + at) = lo;
+  sweep([&](float (&q)[4], int r, int c) {
+    if (r >= o.rows) return;
+    half4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { half_t a, b; split((float)((double)q[e] * inv), a, b); h[e] = a; l[e] = b; }
+    if (!tall) {                                        // (zeros up to the fourth: NP is a multiple of 64)
+      const int at = xat(r, c >> 3) + (c & 7) * 2;
+      *reinterpret_cast<half4*>(X + at) = h;
+      *reinterpret_cast<half4*>(X + xplane + at) = l;
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {                       // (rows beyond m are zero: MP is a multiple of 16)
+      const int at = xat(c + e, r >> 3) + (r & 7) * 2;
+      *reinterpret_cast<half_t*>(X + at) = h[e];
+      *reinterpret_cast<half_t*>(X + xplane + at) = l[e];
+    }
   });
   __syncthreads();
 
@@ -871,34 +897,33 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
 #pragma unroll
       for (int k = 0; k < NT; ++k) acc[k] = mfma4(f[Tri::p[H][k]], f[Tri::q[H][k]], acc[k]);
     }
-    if (quarter) {
+    // tile k is finished by the wave of quarter k & 3: the other three leave it their sums
+    auto slot = [&](int u, int k) { return reinterpret_cast<f32x4*>(R + ((u * TRI + H * Tri::n[0] + k) * 64 + lane) * 16); };
 #pragma unroll
-      for (int k = 0; k < NT; ++k) *reinterpret_cast<f32x4*>(R + (((quarter - 1) * TRI + H * Tri::n[0] + k) * 64 + lane) * 16) = acc[k];
-    }
+    for (int k = 0; k < NT; ++k)
+      if ((k & 3) != quarter) *slot((quarter - k - 1) & 3, k) = acc[k];
     __syncthreads();
-    if (!quarter) {
 #pragma unroll
-      for (int k = 0; k < NT; ++k)
+    for (int k = 0; k < NT; ++k)
+      if ((k & 3) == quarter)
 #pragma unroll
-        for (int u = 0; u < 3; ++u) acc[k] += *reinterpret_cast<const f32x4*>(R + ((u * TRI + H * Tri::n[0] + k) * 64 + lane) * 16);
-    }
+        for (int u = 0; u < 3; ++u) acc[k] += *slot(u, k);
     __syncthreads();
-    if (!quarter) {
 #pragma unroll
-      for (int k = 0; k < NT; ++k) {
-        const int i = 16 * Tri::q[H][k] + li, j = 16 * Tri::p[H][k] + 4 * lg;
-        float v[4];
-        half4 h, l;
+    for (int k = 0; k < NT; ++k) {
+      if ((k & 3) != quarter) continue;
+      const int i = 16 * Tri::q[H][k] + li, j = 16 * Tri::p[H][k] + 4 * lg;
+      float v[4];
+      half4 h, l;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[k][e] * (kOrthInv * kOrthInv);
-        put4(R + aat(i, j >> 3) + (j & 7) * 2, aplane, v, h, l);
-        if (Tri::p[H][k] != Tri::q[H][k]) {
+      for (int e = 0; e < 4; ++e) v[e] = acc[k][e] * (kOrthInv * kOrthInv);
+      put4(R + aat(i, j >> 3) + (j & 7) * 2, aplane, v, h, l);
+      if (Tri::p[H][k] != Tri::q[H][k]) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int at = aat(j + e, i >> 3) + (i & 7) * 2;
-            *reinterpret_cast<half_t*>(R + at) = h[e];
-            *reinterpret_cast<half_t*>(R + aplane + at) = l[e];
-          }
+        for (int e = 0; e < 4; ++e) {
+          const int at = aat(j + e, i >> 3) + (i & 7) * 2;
+          *reinterpret_cast<half_t*>(R + at) = h[e];
+          *reinterpret_cast<half_t*>(R + aplane + at) = l[e];
         }
       }
     }
@@ -954,13 +979,10 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
       for (int r = 0; r < MT; ++r)
 #pragma unroll
         for (int p = 0; p < 2; ++p) b[kk][r][p] = *reinterpret_cast<const half8*>(R + p * aplane + aat(16 * r + li, kk * 4 + lg));
-    for (int jb = wid; jb < NP / 16; jb += 8) {
-      f32x4 acc[MT];
+    half8 f[KK][2], next[KK][2];
+    auto columns = [&](int jb, half8 (&f)[KK][2]) {
 #pragma unroll
-      for (int r = 0; r < MT; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        half8 f[2];
+      for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           typedef __attribute__((address_space(3))) bf16x4* lptr;
@@ -968,11 +990,23 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
           const half4 lo = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lptr)(X + p * xplane + xat(k, j >> 3) + (j & 7) * 2)));
           const half4 hi = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lptr)(X + p * xplane + xat(k + 4, j >> 3) + (j & 7) * 2)));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { f[p][e] = lo[e]; f[p][4 + e] = hi[e]; }
+          for (int e = 0; e < 4; ++e) { f[kk][p][e] = lo[e]; f[kk][p][4 + e] = hi[e]; }
         }
+    };
+    if (wid < NP / 16) columns(wid, f);
+    for (int jb = wid; jb < NP / 16; jb += 8) {
+      if (jb + 8 < NP / 16) columns(jb + 8, next);
+      f32x4 acc[MT];
 #pragma unroll
-        for (int r = 0; r < MT; ++r) acc[r] = mfma4(f, b[kk][r], acc[r]);
-      }
+      for (int r = 0; r < MT; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int r = 0; r < MT; ++r) acc[r] = mfma4(f[kk], b[kk][r], acc[r]);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) f[kk][p] = next[kk][p];
 #pragma unroll
       for (int r = 0; r < MT; ++r) {
         const int i = 16 * r + li, j = jb * 16 + 4 * lg;
