@@ -392,7 +392,8 @@ int pwr_sgd_step(float* p, const float* g, float* buf, long long n, float lr, fl
  * [rows][K]: the K most likely pixels in order, equal ones by the lowest index; K <= 32, 0 = none (both may be NULL).
  * A pixel with s = -inf has no probability, like a masked one.  A row without any: log likelihood -inf, entropy 0, no alternatives (-inf, -1), zero
  * gradient.  What is masked may hold NaN or inf; a NaN or +inf that is allowed makes its row's results NaN.
- * PWR_EUNSUPPORTED: K > 32, or K > 4096 / pieces for a row of V > 16384 values, which is worked on in ceil(V / 16384) pieces or more.
+ * PWR_EUNSUPPORTED: K > 32, or K ceil(V / 16384) > 4096, or a launch of 2^32 threads: 64 per row of up to 512 values, 256 - 1024 per row of up to
+ * 16384 (per piece of longer ones).
  * ------------------------------------------------------------------------------------------- */
 size_t pwr_likelihood_workspace_bytes(long long rows, int V, int K);
 int pwr_likelihood_fwd(const void* z, long long ldz, const float* w, int J, const float* mask, int mask_rows, const long long* index,
@@ -408,7 +409,7 @@ int pwr_likelihood_bwd(const void* z, long long ldz, const float* w, int J, cons
 /* ---------------------------------------------------------------------------------------------
  * Newton-Schulz orthogonalisation: X = G / (|G|_F + eps); `steps` times A = X X^T, X = a X + (b A + c A A) X; out = X.
  * x: `batch` matrices [rows][cols] of `dtype` at any strides >= 0 (elements), entries of a row neighbours; out: contiguous, may be x if x is.
- * rows, cols <= 2^20, rows * cols < 2^31.  The coefficients have to keep every singular value in [0, 1] below 8 (the default quintic: 1.21).
+ * rows, cols <= 2^20, rows * cols < 2^31, batch < 2^22 of the smallest matrices (a launch has less than 2^32 threads; else PWR_EUNSUPPORTED).  The coefficients have to keep every singular value in [0, 1] below 8 (the default quintic: 1.21).
  * ------------------------------------------------------------------------------------------- */
 size_t pwr_orthogonalize_workspace_bytes(int rows, int cols, long long batch);
 int pwr_orthogonalize(const void* x, long long x_batch_stride, long long x_row_stride, void* out, int rows, int cols, long long batch, int dtype,

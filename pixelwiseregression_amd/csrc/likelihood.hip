@@ -626,20 +626,23 @@ __global__ __launch_bounds__(256) void like_gw_kernel(const float* __restrict__ 
 using namespace pwr;
 
 // Values per workgroup of a row that is split: as many as the registers of 512 threads hold -- but a few long rows do not fill 256 CUs that way, so
-// the chunk is halved (down to 4096) until the launch has 256 workgroups.
-static int like_chunk(long long rows, int V) {
+// the chunk is halved (down to 4096) until the launch has 256 workgroups, as long as a row's alternatives still fit the join.
+constexpr int kLikeJoin = 4096;         // candidates of all chunks of a row
+static int like_chunk(long long rows, int V, int K) {
   int c = kLikeChunk;
-  while (V > c && c > 4096 && rows * ((V + c - 1) / c) < 256) c >>= 1;
+  while (V > c && c > 4096 && rows * ((V + c - 1) / c) < 256 && (V + c / 2 - 1) / (c / 2) * (long long)K <= kLikeJoin) c >>= 1;
   return c;
 }
-static int like_chunks(long long rows, int V) {
-  const int c = like_chunk(rows, V);
-  return (V + c - 1) / c;
+static int like_chunks(long long rows, int V, int K) {
+  const int c = like_chunk(rows, V, K);
+  return (int)((V + (long long)c - 1) / c);
 }
+// a launch has at most 2^32 - 1 threads
+static bool like_fits(long long blocks, int threads) { return blocks * threads <= 0xffffffffll; }
 
 extern "C" size_t pwr_likelihood_workspace_bytes(long long rows, int V, int K) {
   if (rows <= 0 || V <= 0 || K < 0) return 0;
-  const int n = like_chunks(rows, V);
+  const int n = like_chunks(rows, V, K);
   return n == 1 ? 0 : (size_t)rows * n * (16 + 8 * (size_t)K);
 }
 
@@ -647,6 +650,7 @@ template <typename T, bool TOP>
 static int like_forward(const LikeArgs& a, hipStream_t s) {
   const long long rows = a.rows;
   if (a.V <= kLikeWaveMax) {
+    if (!like_fits((rows + 3) / 4, 256)) return PWR_EUNSUPPORTED;
     const dim3 g((unsigned)((rows + 3) / 4));
     if (a.V <= 64) hipLaunchKernelGGL((like_fwd_wave_kernel<T, 1>), g, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((like_fwd_wave_kernel<T, 8>), g, dim3(256), 0, s, a);
@@ -655,10 +659,12 @@ static int like_forward(const LikeArgs& a, hipStream_t s) {
   constexpr int N = 16 / sizeof(T);
   if constexpr (!TOP) {
     if (a.V > 4096 && (rows >= kLikeWalkRows || a.chunks == 1)) {
+      if (!like_fits(rows, 256)) return PWR_EUNSUPPORTED;
       hipLaunchKernelGGL((like_walk_kernel<T, 256, 16>), dim3((unsigned)rows), dim3(256), 0, s, a);
       return (int)hipGetLastError();
     }
   }
+  if (!like_fits(rows * a.chunks, a.V <= 256 * N ? 256 : 1024)) return PWR_EUNSUPPORTED;
   const dim3 g((unsigned)(rows * a.chunks));
   if (a.chunks == 1) {
     if (a.V <= 256 * N) hipLaunchKernelGGL((like_fwd_kernel<T, 256, N, false, TOP>), g, dim3(256), 0, s, a);
@@ -682,9 +688,10 @@ extern "C" int pwr_likelihood_fwd(const void* z, long long ldz, const float* w, 
   if (!z || rows < 0 || V <= 0 || K < 0 || J <= 0 || mask_rows <= 0 || ldz < 0 || (K && (!top_logp || !top_index))) return PWR_EINVAL;
   if (dtype != PWR_F32 && dtype != PWR_BF16) return PWR_EINVAL;
   LikeArgs a = {z, ldz, w, J, mask, mask_rows, index, rows, V, K, logp, entropy, stats, top_logp, top_index, 1, V, nullptr, nullptr, nullptr};
-  a.chunk = like_chunk(rows, V);
-  a.chunks = like_chunks(rows, V);
-  if (K > kLikeMaxTop || (long long)a.chunks * K > 4096 || rows * a.chunks > 0x7fffffffll) return PWR_EUNSUPPORTED;
+  if (K > kLikeMaxTop) return PWR_EUNSUPPORTED;
+  a.chunk = like_chunk(rows, V, K);
+  a.chunks = like_chunks(rows, V, K);
+  if ((long long)a.chunks * K > kLikeJoin || rows * a.chunks > 0x7fffffffll) return PWR_EUNSUPPORTED;
   if (a.chunks > 1) {
     if (!workspace || workspace_bytes < pwr_likelihood_workspace_bytes(rows, V, K)) return PWR_ENOSPACE;
     a.part = (float*)workspace;
@@ -716,7 +723,7 @@ extern "C" int pwr_likelihood_bwd(const void* z, long long ldz, const float* w, 
   if (rows < 0 || V <= 0 || J <= 0 || mask_rows <= 0 || ldz < 0 || (rows && (!z || !stats || !entropy || !gz)) || (gw && (!w || rows % J))) return PWR_EINVAL;
   if (dtype != PWR_F32 && dtype != PWR_BF16) return PWR_EINVAL;
   LikeBwdArgs a = {z, ldz, w, J, mask, mask_rows, index, stats, entropy, glogp, gentropy, gz, nullptr, rows, V, like_bwd_chunks(V)};
-  if (rows * a.chunks > 0x7fffffffll) return PWR_EUNSUPPORTED;
+  if (!like_fits(V <= kLikeWaveMax ? (rows + 3) / 4 : rows * a.chunks, 256)) return PWR_EUNSUPPORTED;
   if (gw) {
     if (rows && (!workspace || workspace_bytes < pwr_likelihood_bwd_workspace_bytes(rows, V))) return PWR_ENOSPACE;
     a.gw_part = (float*)workspace;

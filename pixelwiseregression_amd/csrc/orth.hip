@@ -1135,6 +1135,7 @@ static int orth_run(const OrthArgs& g, const OrthCounts& n, const int4* const (&
 
 constexpr int kOrthMaxSide = 1 << 20;
 constexpr int kOrthMaxSteps = 64;
+constexpr long long kOrthMaxBlocks = 0xffffffffll / 1024;         // a launch has at most 2^32 - 1 threads
 
 static bool orth_shape_ok(long long rows, long long cols) {
   // (a matrix of up to 2^31 entries: tile counts and the entries of a plane's row stay in 32 bits, offsets are 64)
@@ -1170,7 +1171,7 @@ static int orthogonalize(const void* x, long long x_batch, long long x_ld, void*
   g.one.first = (int)(sym * shares);
   const OrthCounts n = {{batch * per[0], batch * per[1], batch * sym, batch * per[3], batch * sym * shares}, g.one.Np, g.one.Mp};
   for (const long long k : n.n)
-    if (k > 0x7fffffffll) return PWR_EUNSUPPORTED;
+    if (k > kOrthMaxBlocks) return PWR_EUNSUPPORTED;
   g.shared = shares > 1 && g.one.Mp > kOrthNarrow ? (int)n.n[4] : 0;
   g.slab = (f32x4*)(g.ws + batch * g.ws_stride);
   const int4* const lists[5] = {};
@@ -1180,7 +1181,6 @@ static int orthogonalize(const void* x, long long x_batch, long long x_ld, void*
   const OrthTensor<T> src = {(const T*)x, x_ld};
   const OrthOut<T> dst = {(T*)out, cols};
   if (orth_is_small(rows, cols)) {
-    if (batch > 0x7fffffffll) return PWR_EUNSUPPORTED;
     g.per = 1;
     const dim3 grid((unsigned)batch), block(512);
     const int m = std::min(rows, cols), np = up(std::max(rows, cols), 64);
@@ -1288,7 +1288,7 @@ bool muon_layout(const pwr_muon_param* params, int n, MuonHead& h, std::vector<O
   h.at_rest = take(h.rest * (long long)sizeof(longlong2));
   h.bytes = at;
   for (int k = 0; k < 5; ++k)
-    if (h.n[k] > 0x7fffffffll) return false;
+    if (h.n[k] > kOrthMaxBlocks) return false;
   return h.rest <= 0x7fffffffll;
 }
 

@@ -149,3 +149,26 @@ def test_train_step_refuses():
         TrainStep(m, opt="lion")
     with pytest.raises(ValueError, match="softmax"):
         TrainStep(m, lambda_nll=0.1)
+
+
+def test_launches_beyond_what_the_card_takes_are_refused():
+    l = _lib.lib()
+    assert likelihood(rows=2 ** 26, V=10) == EUNSUPPORTED                                  # 2^32 threads: a wave per row
+    assert likelihood(rows=2 ** 24, V=600) == EUNSUPPORTED and likelihood(rows=2 ** 22, V=3000) == EUNSUPPORTED
+    assert likelihood(rows=2 ** 24, V=20000, ws=SOME, wsb=2 ** 62) == EUNSUPPORTED
+    assert likelihood(rows=2 ** 21, V=20000, K=1, top_logp=SOME, top_index=SOME, ws=SOME, wsb=2 ** 62) == EUNSUPPORTED
+    bwd = lambda rows, V: l.pwr_likelihood_bwd(SOME, 8, None, 1, None, 1, None, SOME, SOME, None, None, SOME, None, rows, V, 0, None, 0, None)  # noqa: E731
+    assert bwd(2 ** 26, 10) == EUNSUPPORTED and bwd(2 ** 24, 600) == EUNSUPPORTED and bwd(2 ** 20, 16 * 4096) == EUNSUPPORTED
+    orth = lambda rows, cols, batch: l.pwr_orthogonalize(SOME, 0, cols, SOME, rows, cols, batch, 0, 5, 1.5, -.5, 0., 1e-7, SOME, 2 ** 62, None)  # noqa: E731
+    assert orth(3, 4, 2 ** 22) == EUNSUPPORTED and orth(128, 128, 2 ** 21) == EUNSUPPORTED and orth(65, 70, 2 ** 40) == EUNSUPPORTED
+
+
+def test_a_lone_long_row_keeps_its_alternatives():
+    """A row is split no further than its alternatives can be joined."""
+    l = _lib.lib()
+    for V in (2 ** 19, 2 ** 20, 2 ** 21):
+        for K in (1, 16, 17, 32):
+            need = l.pwr_likelihood_workspace_bytes(1, V, K)
+            pieces = need // (16 + 8 * K)
+            assert need % (16 + 8 * K) == 0 and pieces * K <= 4096 and V // 16384 <= pieces <= V // 4096
+            assert likelihood(rows=1, V=V, K=K, top_logp=SOME, top_index=SOME, ws=SOME, wsb=need - 1) == ENOSPACE      # (as far as the last check)
