@@ -228,7 +228,7 @@ class LogLikelihoodFn(torch.autograd.Function):
     def forward(ctx, z, w, index, mask, topk):
         r = _Rows(z, index, w, mask)
         logp, entropy, top_logp, top_index, stats = _likelihood_forward(r, topk, True)
-        ctx.save_for_backward(z, w, stats, entropy)      # (z and w: so that a change of either before the backward pass is noticed)
+        ctx.save_for_backward(z, w, index, mask, stats, entropy)     # (the inputs: so that a change of one before the backward pass is noticed)
         ctx.r = r                                        # inputs and copies of inputs only: no cycle through an output
         ctx.set_materialize_grads(False)
         if topk:
@@ -238,7 +238,7 @@ class LogLikelihoodFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, glogp, gentropy, _, __):
-        z, w, stats, entropy = ctx.saved_tensors
+        z, w, _, _, stats, entropy = ctx.saved_tensors
         if glogp is None and gentropy is None:
             return None, None, None, None, None
         need_z, need_w = ctx.needs_input_grad[:2]
@@ -255,10 +255,11 @@ def log_likelihood(z, index, w=None, mask=None, topk=0):
 
     z: logits ``[B, J, H, W]``, ``[B, J, V]`` or ``[N, V]``, float32 or bfloat16.  index: ``[B, J]`` (``[N]``) whole numbers, -1 where no pixel is
     given (log likelihood 0, no gradient); a pixel outside its map gives NaN; None: no ``logp``.  w: one number per joint.  mask: ``[B, 1, H, W]``
-    (one per sample) or one per map; 0 = not allowed, whatever z holds there.  topk <= 32: equal values go by the lowest index; what does not exist
+    (one per sample) or one per map; 0 = not allowed, whatever z holds there.  topk <= 32 (less for maps of over 2^21 pixels): equal values go by the lowest index; what does not exist
     (masked, -inf, beyond the map) is ``(-inf, -1)``.  A map without an allowed pixel: -inf, entropy 0, zero gradient.
 
-    Returns ``LogLikelihood(logp, entropy, top_logp, top_index)``, float32 (int64 the last); gradients of ``logp`` and ``entropy`` reach z and w."""
+    Returns ``LogLikelihood(logp, entropy, top_logp, top_index)``, float32 (int64 the last); gradients of ``logp`` and ``entropy`` reach z and w.
+    In a captured graph: ``likelihood_gradients``, or forward and backward with no other autograd graph of the same leaves alive."""
     _require_cuda(z, index, w, mask)
     topk = int(topk)
     if not 0 <= topk <= 32:
@@ -295,6 +296,14 @@ def heatmap_pixels(uvd, P):
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
+def _overlap(s, t):
+    """Whether the spans of memory of two tensors meet."""
+    def span(u):
+        return u.data_ptr(), u.data_ptr() + (1 + sum((n - 1) * k for n, k in zip(u.shape, u.stride()))) * u.element_size()
+    (a, b), (c, d) = span(s), span(t)
+    return s.numel() > 0 and t.numel() > 0 and s.device == t.device and a < d and c < b
+
+
 def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
     """The matrices ``x`` (``[..., rows, cols]``, float32 or bfloat16) made nearly orthogonal by ``steps`` Newton-Schulz products:
     ``X = x / (|x| + eps)``, then ``X = a X + (b A + c A A) X`` with ``A = X X^T`` (of the shorter side).  With the default coefficients every singular
@@ -315,6 +324,8 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
         out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous %s tensor of shape %s" % (x.dtype, tuple(x.shape)))
+    elif _overlap(x, out) and not (out.data_ptr() == x.data_ptr() and x.is_contiguous()):
+        raise ValueError("out shares memory with x: it has to be x itself, contiguous, or apart from it")
     _same_device(x, out)
     if x.numel() == 0:
         return out

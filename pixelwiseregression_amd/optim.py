@@ -6,7 +6,8 @@ choice of ``TrainStep(opt=...)``.
 
 Matrices -- the conv kernels, one row per output channel -- take the orthogonalised momentum (``ops.orthogonalize``) scaled to the rms an AdamW
 update has (``update_rms``, so one learning rate serves both); every other parameter takes an AdamW step.  All parameters of a network go through the
-same seventeen launches, whatever their number and shapes.
+same few launches (eighteen; more where some of them are long), whatever their number and shapes.  A step that is captured into a graph keeps the
+learning rate and the step number it was captured with.
 """
 import ctypes
 

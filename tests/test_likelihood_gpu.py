@@ -117,6 +117,23 @@ def test_alternatives(K, V):
     check(*inputs(2, 2, V, w=False, seed=K), topk=K, grads=False)
 
 
+@pytest.mark.parametrize("K,V", [(17, 2 ** 20), (32, 2 ** 21), (32, 600001)])
+def test_alternatives_of_one_long_row(K, V):
+    check(*inputs(1, 1, V, w=False, seed=K), topk=K, grads=False)
+
+
+def test_a_changed_input_is_noticed():
+    from pixelwiseregression_amd import ops
+    for changed in range(4):
+        z, index, w, m = (t.to(DEV) for t in inputs(4, 3, 100, mask="sample", seed=1))
+        q, v = z.clone().requires_grad_(), w.clone().requires_grad_()
+        r = ops.log_likelihood(q, index, v, m)
+        with torch.no_grad():
+            (q, v, index, m)[changed].zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(r.entropy.sum(), [q, v])
+
+
 @pytest.mark.parametrize("V", [50, 512, 3000, 16384, 30000])
 def test_ties_go_to_the_lowest_index(V):
     # every value equal; two values only; bf16 values of a coarse grid: more candidates than the selection sorts at once

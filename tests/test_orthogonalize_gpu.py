@@ -141,6 +141,20 @@ def test_strides_results_and_in_place(dtype):
     assert ops.orthogonalize(base[:0]).shape == (0, 60, 90) and ops.orthogonalize(base[:, :0]).shape == (5, 0, 90)
 
 
+def test_a_result_that_overlaps_is_refused():
+    from pixelwiseregression_amd import ops
+    store = torch.randn(4, 5, 6, device=DEV)
+    for x, out in ((store[:3], store[1:]), (store[:1].expand(3, 5, 6), store[:3]), (store[0, :, :5].T, store[0, :, :5].T)):
+        with pytest.raises(ValueError):
+            ops.orthogonalize(x, out=out)
+    square = torch.randn(6, 6, device=DEV)
+    with pytest.raises(ValueError):
+        ops.orthogonalize(square.T, out=square)
+    want = ops.orthogonalize(store[1])
+    ops.orthogonalize(store[1], out=store[2])                 # neighbours
+    assert torch.equal(store[2], want)
+
+
 def test_a_strided_batch_in_both_tiles():
     """The source's batch and row strides are the caller's, the result's are not (also with enough matrices for the wide tile)."""
     from pixelwiseregression_amd import ops
