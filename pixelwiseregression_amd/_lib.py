@@ -83,5 +83,10 @@ def ptr(t):
 
 
 def stream_ptr(device=None):
+    """The handle of the current stream of ``device`` (a torch.device; None: the current one)."""
     import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    index = getattr(device, "index", None)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)          # (without a Stream object on the way: 0.2 us instead of 2)
+    if raw is None or index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return raw(index)
