@@ -5,7 +5,8 @@ Public surface mirrors the reference's ``model.py`` / ``utils.py`` names for the
 (datasets.py:100), ``save_model`` / ``load_model`` (utils.py:302-314), ``make_targets`` (the dense targets of
 datasets.py:285-294 / :365-383, on the device), ``preprocess_batch`` (the crop / resize / augmentation pipeline of
 datasets.py:243-299 for a batch of raw depth frames in HBM), ``StreamedInference`` (the evaluation loop of test.py:93-102 with two
-batches in flight on two HIP streams).
+batches in flight on two HIP streams).  Beyond the reference: ``ops.log_likelihood`` / ``ops.likelihood_gradients`` (likelihood, entropy and most
+likely pixels of a heat map), ``ops.orthogonalize``, and ``optim.Muon``, the optimizer built on it.
 """
 from .model import PixelwiseRegression  # noqa: F401
 from .metric import recover_uvd, uvd2xyz, mean_joint_error, INTRINSICS  # noqa: F401

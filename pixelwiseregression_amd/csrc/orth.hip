@@ -1054,14 +1054,26 @@ static OrthItem orth_make(int rows, int cols, int tile) {
 static long long orth_sym_tiles(const OrthItem& o, int tile) { const long long t = o.Mp / tile; return t * (t + 1) / 2; }
 static long long orth_apply_tiles(const OrthItem& o, int tile) { return (long long)(o.Mp / tile) * (o.Np / tile); }
 
-// 128 x 128 tiles move half the bytes per product of 64 x 64 ones; they pay from three tiles a side on, where a launch of them has a workgroup per CU.  One
-// matrix in 128 / 64: 2048 x 2048 fp32 835 / 1020 us, 700 x 7000 475 / 583, 1024 x 4096 469 / 475, 1024 x 2048 398 / 307; 64 of 128 x 1152 341 / 283.
-constexpr int kOrthWideSide = 384, kOrthWideTiles = 256;
+// 128 x 128 tiles move half the bytes per product of 64 x 64 ones, and pad more.  They pay from six tiles a side on, where B X has a tile per CU, by about
+// m / 8192 of the time; that is compared with what padding and a last round of B X (512 places) cost.  In 128 / 64: 2048 x 2048 fp32 854 / 1086 us,
+// 4000 x 8000 bf16 3495 / 5462, 2 of 1000 x 3000 fp32 630 / 728, 1024 x 4096 487 / 521; 1300 x 6000 (517 tiles) 1021 / 878, 900 x 8000 728 / 652,
+// 4 of 640 x 2560 496 / 448, 16 of 400 x 1600 746 / 556, 64 of 128 x 1152 348 / 250.
+constexpr int kOrthWideSide = 705, kOrthWideTiles = 256;
+static double orth_cost(int rows, int cols, long long batch, int tile) {
+  const OrthItem o = orth_make(rows, cols, tile);
+  long long t = batch * orth_apply_tiles(o, tile);
+  if (tile == 128 && t > 512) t = (t + 511) / 512 * 512;
+  const double area = (tile / 64) * (tile / 64);
+  return area * ((double)t * o.Mp + (double)batch * orth_sym_tiles(o, tile) * (o.Np + (double)o.Mp));
+}
 static int orth_tile(int rows, int cols, long long batch) {
-  return std::min(rows, cols) >= kOrthWideSide && batch * orth_apply_tiles(orth_make(rows, cols, 128), 128) >= kOrthWideTiles ? 128 : 64;
+  const int m = std::min(rows, cols);
+  if (m < kOrthWideSide || batch * orth_apply_tiles(orth_make(rows, cols, 128), 128) < kOrthWideTiles) return 64;
+  return orth_cost(rows, cols, batch, 128) * 8192 <= orth_cost(rows, cols, batch, 64) * (8192.0 + m) ? 128 : 64;
 }
 
-// X of such a matrix fits the LDS of one CU
+// X of such a matrix fits the LDS of one CU.  In one workgroup a matrix / by launches: 64 x 128 fp32 24 / 78 us, 64 x 512 59 / 90, 32 x 1024 47 / 92,
+// 600 of 64 x 500 bf16 175 / 374, 2000 of 64 x 128 bf16 193 / 470.
 static bool orth_is_small(int rows, int cols) {
   const long long m = std::min(rows, cols), n = (std::max(rows, cols) + 63ll) / 64 * 64;
   return m <= 32 ? n <= 1024 : m <= 64 && n <= 512;
@@ -1219,7 +1231,7 @@ struct MuonHead {
 };
 constexpr unsigned long long kMuonMagic = 0x32304e4f554d5750ull;
 
-// a list is worked on in the tile that most of its products want (in units of a 64 x 64 x 64 block): the rule of orth_tile
+// a list is worked on in the tile that most of its products want (in units of a 64 x 64 x 64 block), after orth_tile, padding aside
 int muon_tile(const std::vector<OrthItem>& v) {
   double wide = 0, all = 0;
   long long tiles = 0;

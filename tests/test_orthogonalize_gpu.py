@@ -73,7 +73,7 @@ def test_batches(batch, rows, cols, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("batch,rows,cols", [(1, 1100, 4400), (4, 500, 2100), (30, 400, 450), (52, 390, 400), (1, 20, 8000), (3, 2300, 70), (4, 300, 2000),
-                                             (2, 6, 70000)])
+                                             (2, 6, 70000), (28, 760, 768), (2, 2100, 1100)])
 def test_products_split_along_k(batch, rows, cols, dtype):
     """Symmetric products whose tiles do not fill the chip: few of them, a last round of few, small ones with long sums."""
     x = np.random.default_rng(5).standard_normal((batch, rows, cols)).astype(np.float32)
@@ -164,7 +164,17 @@ def test_a_strided_batch_in_both_tiles():
         assert torch.equal(ops.orthogonalize(x), ops.orthogonalize(x.contiguous()))
 
 
-@pytest.mark.parametrize("shape", [(64, 128), (20, 130, 260), (64, 140, 300)])
+def test_strides_of_wide_matrices():
+    from pixelwiseregression_amd import ops
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.randn(2, 1104, 2603, device=DEV).to(dtype)[:, 3:1103, 2:2602]
+        want = ops.orthogonalize(x.contiguous())
+        assert torch.equal(ops.orthogonalize(x), want) and torch.equal(ops.orthogonalize(x), want)
+        y = x.contiguous()
+        assert ops.orthogonalize(y, out=y) is y and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("shape", [(64, 128), (20, 130, 260), (64, 140, 300), (1100, 4400)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_repeats_streams_and_graphs(shape, dtype):
     from pixelwiseregression_amd import ops
@@ -245,7 +255,8 @@ def test_muon_step(kw):
 
 
 @pytest.mark.parametrize("shapes", [[(40, 50)], [(7,)], [(1, 1)], [(3000, 2)], [(128, 128, 3, 3)] * 30 + [(128,)] * 30, [(9,), (0,), (4, 0), (4, 4)], [(400, 1200), (500, 2000), (64, 64), (30,), (1000, 1000), (390, 4000)],
-                                    [(300, 500), (20000,)], [(64, 64), (20, 8000), (9,), (128, 3200), (2100, 60), (3, 100)]])
+                                    [(300, 500), (20000,)], [(64, 64), (20, 8000), (9,), (128, 3200), (2100, 60), (3, 100)],
+                                    [(1000, 2100), (64, 64), (2500, 900), (30,), (20, 400), (1000, 1000)]])
 def test_muon_lists(shapes):
     muon_case(shapes, seed=4)
 
