@@ -356,12 +356,19 @@ __device__ __forceinline__ OrthPair<N> orth_finish(const OrthArgs& g, const Orth
     if constexpr (KIND == kPoly) {
       const float* const da = diag ? diag : dA;
       const float di = TERMS == 1 ? da[i] : 0.f;
+      float dj[N];
+#pragma unroll
+      for (int e = 0; e < N; e += 4) {
+        const f32x4 d = TERMS == 1 ? *reinterpret_cast<const f32x4*>(da + j + e) : f32x4{0.f, 0.f, 0.f, 0.f};
+        dj[e] = d.x; dj[e + 1] = d.y; dj[e + 2] = d.z; dj[e + 3] = d.w;
+      }
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         float aij = ((float)beside.h.v[e] + (float)beside.l.v[e]) * kOrthInv, aa = v[e];
         if constexpr (TERMS == 1) {
-          if (i == j + e) { aij = di; aa = fmaf(di, di, aa); }
-          else aa = fmaf(di + da[j + e], aij, aa);
+          const bool same = i == j + e;
+          aa = fmaf(same ? di : di + dj[e], same ? di : aij, aa);
+          aij = same ? di : aij;
         }
         v[e] = fmaf(g.c, aa, g.b * aij);
       }
@@ -395,7 +402,7 @@ __device__ __forceinline__ void orth_mirror(const OrthArgs& g, const OrthItem& o
 // written out, and multiplies from there.
 template <int TERMS>
 __device__ __forceinline__ void orth_narrow_poly(const OrthArgs& g, const OrthItem& o, const OrthWs& w, int ti, int tj, char* lds) {
-  __shared__ float diag[kOrthNarrow];
+  __shared__ __attribute__((aligned(16))) float diag[kOrthNarrow];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
   const int Mp = o.Mp, plane = Mp * Mp * 2, flip = Mp == 128 ? 15 : 7, shift = Mp == 128 ? 0 : 1;
   // rows of Mp * 2 bytes, their 16-byte units swizzled by the row
@@ -465,14 +472,15 @@ __device__ __forceinline__ void orth_narrow_poly(const OrthArgs& g, const OrthIt
 // A and A A are symmetric: tiles tj >= ti only, written twice.  In B X the columns of X are needed along K: its rows are staged as they are
 // and read transposed by the LDS hardware.
 // TILE 128, large matrices: a wave has (TILE / 2)^2; two stages in LDS, the next one in registers on its way; few tiles, or a last round of few, are split
-// along K over workgroups.
+// along K over workgroups.  2048 x 8192 fp32: A 131 us and its join 10, A A 38 + 12, B X 204 = 1010 TFLOP/s of fp16 products.  4096 x 4096 bf16: A 88, A A
+// 99, B X 168 = 815 TFLOP/s: the LDS reads of 64 x 64 a wave take as long as its matrix instructions.
 // TILE 64, for the few workgroups of smaller ones, where a stage costs its latency.  B X: stages of 64 along K.  A and A A (KG = 4): stages of 128, two on
 // their way in registers, their four steps of 32 shared out over four groups of four waves, which add their sums through LDS.  (Measured and not kept:
 // fragments straight from memory, no LDS along K, 1.4 to 2 times slower; four waves with the whole tile and a step each, 3 - 8 % slower.)
 template <int TERMS, int KIND, int TILE, int KG, typename OUT>
 __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(OrthArgs g, OUT fin, int last) {
   constexpr int NT = 256 * KG;
-    constexpr int KS = TILE == 128 ? (TERMS == 3 ? 32 : 64) : KG == 4 ? 128 : 64;        // K per stage
+  constexpr int KS = TILE == 128 ? (TERMS == 3 ? 32 : 64) : KG == 4 ? 128 : 64;        // K per stage
   constexpr int STAGES = TILE == 128 ? 2 : 1;
   constexpr int SIDE = TILE / 2, NF = SIDE / 16;                        // of a wave's part of the tile; 16 x 16 fragments a side
   constexpr int PLANES = TERMS == 3 ? 2 : 1;
@@ -658,6 +666,11 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
     return;
   }
   const bool mirror = KIND != kApply && ti != tj;
+  // (all loads together: behind one another's stores they would cost a latency each; before the last stages they would cost registers the stages need)
+  if (STAGES == 2) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) beside[r] = orth_beside<KIND, 4 * NP>(g, o, w, i0 + 16 * r, j0);
+  }
   f32x4* sums = reinterpret_cast<f32x4*>(lds);
   if constexpr (KG > 1) {
     __syncthreads();
@@ -692,8 +705,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
       for (int e = 0; e < 4; ++e) v[4 * k + e] = a[e];
     }
     const int i = i0 + 16 * r;
-    const OrthPair<4 * NP> b = STAGES == 1 ? beside[r] : orth_beside<KIND, 4 * NP>(g, o, w, i, j0);
-    const OrthPair<4 * NP> d = orth_finish<TERMS, KIND, 4 * NP, OUT>(g, o, w, fin, last, i, j0, v, b);
+    const OrthPair<4 * NP> d = orth_finish<TERMS, KIND, 4 * NP, OUT>(g, o, w, fin, last, i, j0, v, beside[r]);
     if (!mirror) continue;
     if constexpr (TILE == 128) {
       // row i of the block: 128 bytes per plane, its 16-byte units swizzled
