@@ -315,26 +315,33 @@ struct OrthUpdate {
     if (i >= m) return;
     const float step = lr * o.gain;
     float* base = p + o.dst;
+    constexpr int C = N < 8 ? N : 8;                                  // (sixteen together spill)
     if (!tall && j + N <= n) {
       float* q = base + (long long)i * o.cols + j;
-      Quad<float> x[N / 4];
 #pragma unroll
-      for (int k = 0; k < N / 4; ++k) x[k] = *reinterpret_cast<const Quad<float>*>(q + 4 * k);
+      for (int h = 0; h < N; h += C) {
+        Quad<float> x[C / 4];
 #pragma unroll
-      for (int k = 0; k < N / 4; ++k) {
+        for (int k = 0; k < C / 4; ++k) x[k] = *reinterpret_cast<const Quad<float>*>(q + h + 4 * k);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[k].v[e] = x[k].v[e] * keep - step * v[4 * k + e];
-        *reinterpret_cast<Quad<float>*>(q + 4 * k) = x[k];
+        for (int k = 0; k < C / 4; ++k) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[k].v[e] = x[k].v[e] * keep - step * v[h + 4 * k + e];
+          *reinterpret_cast<Quad<float>*>(q + h + 4 * k) = x[k];
+        }
       }
       return;
     }
     auto at = [&](int jj) { return tall ? (long long)jj * o.cols + i : (long long)i * o.cols + jj; };
-    float x[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = base[at(min(j + e, n - 1))];
+    for (int h = 0; h < N; h += C) {
+      float x[C];
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (j + e < n) base[at(j + e)] = x[e] * keep - step * v[e];
+      for (int e = 0; e < C; ++e) x[e] = base[at(min(j + h + e, n - 1))];
+#pragma unroll
+      for (int e = 0; e < C; ++e)
+        if (j + h + e < n) base[at(j + h + e)] = x[e] * keep - step * v[h + e];
+    }
   }
 };
 struct OrthNone {
@@ -511,8 +518,9 @@ __device__ __forceinline__ void orth_narrow_poly(const OrthArgs& g, const OrthIt
 // TILE 64, for the few workgroups of smaller ones, where a stage costs its latency.  B X: stages of 64 along K.  A and A A (KG = 4): stages of 128, two on
 // their way in registers, their four steps of 32 shared out over four groups of four waves, which add their sums through LDS.  (Measured and not kept:
 // fragments straight from memory, no LDS along K, 1.4 to 2 times slower; four waves with the whole tile and a step each, 3 - 8 % slower.)
+// (Registers for two 128 x 128 workgroups a CU, or four of B X in 64 x 64: with three the 14-joint step takes 168 us instead of 160, with five it spills.)
 template <int TERMS, int KIND, int TILE, int KG, typename OUT>
-__global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(OrthArgs g, OUT fin, int last) {
+__global__ __launch_bounds__(256 * KG, KG > 1 ? 1 : TILE == 64 ? 4 : 2) void orth_gemm_kernel(OrthArgs g, OUT fin, int last) {
   constexpr int NT = 256 * KG;
   constexpr int KS = TILE == 128 ? (TERMS == 3 ? 32 : 64) : KG == 4 ? 128 : 64;        // K per stage
   constexpr int STAGES = TILE == 128 ? 2 : 1;
@@ -700,8 +708,10 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
     return;
   }
   const bool mirror = KIND != kApply && ti != tj;
-  // (all loads together: behind one another's stores they would cost a latency each; before the last stages they would cost registers the stages need)
-  if (STAGES == 2) {
+  // (all loads together: behind one another's stores they would cost a latency each; before the last stages, or beside the parameters of an update, they would
+  // cost registers that are needed)
+  constexpr bool TOGETHER = STAGES == 2 && !std::is_same<OUT, OrthUpdate>::value;
+  if (TOGETHER) {
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) beside[r] = orth_beside<KIND, 4 * NP>(g, o, w, i0 + 16 * r, j0);
   }
@@ -739,6 +749,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void orth_gemm_kernel(Or
       for (int e = 0; e < 4; ++e) v[4 * k + e] = a[e];
     }
     const int i = i0 + 16 * r;
+    if (STAGES == 2 && !TOGETHER) beside[r] = orth_beside<KIND, 4 * NP>(g, o, w, i, j0);
     const OrthPair<4 * NP> d = orth_finish<TERMS, KIND, 4 * NP, OUT>(g, o, w, fin, last, i, j0, v, beside[r]);
     if (!mirror) continue;
     if constexpr (TILE == 128) {
