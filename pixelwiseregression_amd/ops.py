@@ -102,6 +102,7 @@ class _on:
 
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_INT = 2 ** 31 - 1
 
 
 def _dtype_tag(t, what):
@@ -143,12 +144,14 @@ class _Rows:
         self.dtype = _dtype_tag(z, "z")
         self.lead = lead = tuple(shape[:1]) if dim == 2 else tuple(shape[:2])
         self.J = J = shape[1] if dim > 2 else 1
-        v = z.flatten(2) if dim == 4 else z
-        self.rows, self.V = (lead[0] * J if dim > 2 else lead[0]), v.shape[-1]
+        self.rows, self.V = (lead[0] * J if dim > 2 else lead[0]), shape[-1] * shape[-2] if dim == 4 else shape[-1]
         if self.V < 1:
             raise ValueError("a row of no values")
         if J < 1:
             raise ValueError("no joints")
+        if self.V > _INT or J > _INT:                    # (they cross the C ABI as int, which would cut them)
+            raise ValueError("rows of %d values, %d joints: 2^31 - 1 at most" % (self.V, J))
+        v = z.flatten(2) if dim == 4 else z
         if not v.is_contiguous():
             if (self.V > 1 and v.stride(-1) != 1) or (v.dim() == 3 and v.shape[0] > 1 and J > 1 and v.stride(0) != J * v.stride(1)):
                 v = v.contiguous()
@@ -320,6 +323,9 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
     steps = int(steps)
     if not 1 <= steps <= 64 or not float(eps) >= 0.0:
         raise ValueError("steps must be 1 .. 64 and eps not negative, got %d, %g" % (steps, eps))
+    rows, cols = x.shape[-2:]
+    if x.numel() and (max(rows, cols) > 2 ** 20 or rows * cols > _INT):      # (before they cross the C ABI as int, which would cut them)
+        raise ValueError("matrices of %d x %d are larger than orthogonalize takes (2^20 a side, 2^31 - 1 entries)" % (rows, cols))
     if out is None:
         out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
@@ -329,14 +335,11 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
     _same_device(x, out)
     if x.numel() == 0:
         return out
-    rows, cols = x.shape[-2:]
     v = x if x.dim() == 3 else x.reshape(-1, rows, cols)
     if (cols > 1 and v.stride(2) != 1) or (v is not x and v.data_ptr() != x.data_ptr()):
         v = v.contiguous()
     l = _lib.lib()
     need = l.pwr_orthogonalize_workspace_bytes(rows, cols, v.shape[0])
-    if need == 0:
-        raise ValueError("matrices of %d x %d are larger than orthogonalize takes (2^20 a side, 2^31 entries)" % (rows, cols))
     ws = torch.empty(need, device=x.device, dtype=torch.uint8)
     with _on(x.device):
         _lib.check(l.pwr_orthogonalize(v.data_ptr(), v.stride(0), v.stride(1), out.data_ptr(), rows, cols, v.shape[0], tag, steps, a, b, c, float(eps),
