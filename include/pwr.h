@@ -392,7 +392,7 @@ int pwr_sgd_step(float* p, const float* g, float* buf, long long n, float lr, fl
  * [rows][K]: the K most likely pixels in order, equal ones by the lowest index; K <= 32, 0 = none (both may be NULL).
  * A pixel with s = -inf has no probability, like a masked one.  A row without any: log likelihood -inf, entropy 0, no alternatives (-inf, -1), zero
  * gradient.  What is masked may hold NaN or inf; a NaN or +inf that is allowed makes its row's results NaN.
- * PWR_EUNSUPPORTED: K > 32, or K ceil(V / 16384) > 4096, or a launch of 2^32 threads: 64 per row of up to 512 values, 256 - 1024 per row of up to
+ * PWR_EUNSUPPORTED: K > 32, or K ceil(V / 16384) > 4096, or V > 2^31 - 2^14, or a launch of 2^32 threads: 64 per row of up to 512 values, 256 - 1024 per row of up to
  * 16384 (per piece of longer ones).
  * ------------------------------------------------------------------------------------------- */
 size_t pwr_likelihood_workspace_bytes(long long rows, int V, int K);

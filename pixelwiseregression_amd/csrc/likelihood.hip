@@ -26,6 +26,7 @@ constexpr int kLikeChunk = 16384;       // values of a row one workgroup holds i
 // rows than this.  Walked / split: 512 rows of 50001 fp32 18.6 / 24.0 us, bf16 19.6 / 22.2; 256 rows 13.0 / 15.4 and 15.3 / 13.9.
 constexpr int kLikeWalkRows = 512;
 constexpr int kLikeWaveMax = 512;       // rows up to here: one wave per row (64 lanes x 8)
+constexpr int kLikeMaxRow = 0x7fffffff - kLikeChunk + 1;       // 2^31 - 2^14: the end of a row's last piece is an int too
 
 struct LikeArgs {
   const void* z; long long ldz;         // [rows] of V values, ldz apart
@@ -638,10 +639,12 @@ static int like_chunks(long long rows, int V, int K) {
   return (int)((V + (long long)c - 1) / c);
 }
 // a launch has at most 2^32 - 1 threads
-static bool like_fits(long long blocks, int threads) { return blocks * threads <= 0xffffffffll; }
+static bool like_fits(long long blocks, int threads) { return blocks <= 0xffffffffll / threads; }
+// what the kernels count in 32 bits (and no product of the checks below leaves 64)
+static bool like_countable(long long rows, int V) { return rows <= 0xffffffffll && V <= kLikeMaxRow; }
 
 extern "C" size_t pwr_likelihood_workspace_bytes(long long rows, int V, int K) {
-  if (rows <= 0 || V <= 0 || K < 0) return 0;
+  if (rows <= 0 || V <= 0 || K < 0 || !like_countable(rows, V)) return 0;
   const int n = like_chunks(rows, V, K);
   return n == 1 ? 0 : (size_t)rows * n * (16 + 8 * (size_t)K);
 }
@@ -688,7 +691,7 @@ extern "C" int pwr_likelihood_fwd(const void* z, long long ldz, const float* w, 
   if (!z || rows < 0 || V <= 0 || K < 0 || J <= 0 || mask_rows <= 0 || ldz < 0 || (K && (!top_logp || !top_index))) return PWR_EINVAL;
   if (dtype != PWR_F32 && dtype != PWR_BF16) return PWR_EINVAL;
   LikeArgs a = {z, ldz, w, J, mask, mask_rows, index, rows, V, K, logp, entropy, stats, top_logp, top_index, 1, V, nullptr, nullptr, nullptr};
-  if (K > kLikeMaxTop) return PWR_EUNSUPPORTED;
+  if (K > kLikeMaxTop || !like_countable(rows, V)) return PWR_EUNSUPPORTED;
   a.chunk = like_chunk(rows, V, K);
   a.chunks = like_chunks(rows, V, K);
   if ((long long)a.chunks * K > kLikeJoin || rows * a.chunks > 0x7fffffffll) return PWR_EUNSUPPORTED;
@@ -705,7 +708,9 @@ extern "C" int pwr_likelihood_fwd(const void* z, long long ldz, const float* w, 
 
 static int like_bwd_chunks(int V) { return V <= kLikeWaveMax ? 1 : (V + kLikeBwdChunk - 1) / kLikeBwdChunk; }
 
-extern "C" size_t pwr_likelihood_bwd_workspace_bytes(long long rows, int V) { return rows <= 0 || V <= 0 ? 0 : (size_t)rows * like_bwd_chunks(V) * 4; }
+extern "C" size_t pwr_likelihood_bwd_workspace_bytes(long long rows, int V) {
+  return rows <= 0 || V <= 0 || !like_countable(rows, V) ? 0 : (size_t)rows * like_bwd_chunks(V) * 4;
+}
 
 template <typename T>
 static void like_backward(const LikeBwdArgs& a, hipStream_t s) {
@@ -722,6 +727,7 @@ extern "C" int pwr_likelihood_bwd(const void* z, long long ldz, const float* w, 
   if (rows == 0 && !gw) return 0;
   if (rows < 0 || V <= 0 || J <= 0 || mask_rows <= 0 || ldz < 0 || (rows && (!z || !stats || !entropy || !gz)) || (gw && (!w || rows % J))) return PWR_EINVAL;
   if (dtype != PWR_F32 && dtype != PWR_BF16) return PWR_EINVAL;
+  if (!like_countable(rows, V)) return PWR_EUNSUPPORTED;
   LikeBwdArgs a = {z, ldz, w, J, mask, mask_rows, index, stats, entropy, glogp, gentropy, gz, nullptr, rows, V, like_bwd_chunks(V)};
   if (!like_fits(V <= kLikeWaveMax ? (rows + 3) / 4 : rows * a.chunks, 256)) return PWR_EUNSUPPORTED;
   if (gw) {

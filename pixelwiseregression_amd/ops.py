@@ -103,6 +103,7 @@ class _on:
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _INT = 2 ** 31 - 1
+_LONGEST_ROW = 2 ** 31 - 2 ** 14
 
 
 def _dtype_tag(t, what):
@@ -149,8 +150,8 @@ class _Rows:
             raise ValueError("a row of no values")
         if J < 1:
             raise ValueError("no joints")
-        if self.V > _INT or J > _INT:                    # (they cross the C ABI as int, which would cut them)
-            raise ValueError("rows of %d values, %d joints: 2^31 - 1 at most" % (self.V, J))
+        if self.V > _LONGEST_ROW or J > _INT:            # (they cross the C ABI as int, which would cut them)
+            raise ValueError("rows of %d values (2^31 - 2^14 at most), %d joints (2^31 - 1)" % (self.V, J))
         v = z.flatten(2) if dim == 4 else z
         if not v.is_contiguous():
             if (self.V > 1 and v.stride(-1) != 1) or (v.dim() == 3 and v.shape[0] > 1 and J > 1 and v.stride(0) != J * v.stride(1)):
