@@ -34,7 +34,7 @@ extern "C" {
 #define PWR_HEATMAP_SUM 1     /* model.py:86-90 */
 
 /* ABI version of this header; pwr_abi_version() must return the same number. */
-#define PWR_ABI_VERSION 8   /* 8: pwr_likelihood_*, pwr_orthogonalize, pwr_muon_*, pwr_engine_logits_offset, pwr_engine_logit_grad; 7 (round 6): pwr_conv_dgrad_fold_stats_pair; 6 (round 6): pwr_norm_bwd_apply_from_partial, pwr_norm_bwd_params_from_partial, pwr_norm_bwd_params_group, pwr_norm_finalize_partial_pair, pwr_engine_pack_beside_forward, pwr_norm_apply, pwr_norm_stats_fused_src, pwr_nchw_to_nhwc_pad_pair; 5 (round 5): pwr_conv_fwd_nchw_pair, the order field of the pack records and the tag bit of a fragment-order pack; 4 (round 4): pwr_conv_dgrad_stats_pair, pwr_conv_wgrad_pair, pwr_engine_wait_segment, pwr_resblock_bwd_small_x, pwr_norm_bwd_from_partial_pair, pwr_conv_fwd_stats mode 1; 3 (round 3): experiment entry points removed, debugging aids moved to pwr_debug.h */
+#define PWR_ABI_VERSION 9   /* 9: pwr_orthogonalize_range; 8: pwr_likelihood_*, pwr_orthogonalize, pwr_muon_*, pwr_engine_logits_offset, pwr_engine_logit_grad; 7 (round 6): pwr_conv_dgrad_fold_stats_pair; 6 (round 6): pwr_norm_bwd_apply_from_partial, pwr_norm_bwd_params_from_partial, pwr_norm_bwd_params_group, pwr_norm_finalize_partial_pair, pwr_engine_pack_beside_forward, pwr_norm_apply, pwr_norm_stats_fused_src, pwr_nchw_to_nhwc_pad_pair; 5 (round 5): pwr_conv_fwd_nchw_pair, the order field of the pack records and the tag bit of a fragment-order pack; 4 (round 4): pwr_conv_dgrad_stats_pair, pwr_conv_wgrad_pair, pwr_engine_wait_segment, pwr_resblock_bwd_small_x, pwr_norm_bwd_from_partial_pair, pwr_conv_fwd_stats mode 1; 3 (round 3): experiment entry points removed, debugging aids moved to pwr_debug.h */
 int pwr_abi_version(void);
 
 /* ---------------------------------------------------------------------------------------------
@@ -409,8 +409,12 @@ int pwr_likelihood_bwd(const void* z, long long ldz, const float* w, int J, cons
 /* ---------------------------------------------------------------------------------------------
  * Newton-Schulz orthogonalisation: X = G / (|G|_F + eps); `steps` times A = X X^T, X = a X + (b A + c A A) X; out = X.
  * x: `batch` matrices [rows][cols] of `dtype` at any strides >= 0 (elements), entries of a row neighbours; out: contiguous, may be x if x is.
- * rows, cols <= 2^20, rows * cols < 2^31, batch < 2^22 of the smallest matrices (a launch has less than 2^32 threads; else PWR_EUNSUPPORTED).  The coefficients have to keep every singular value in [0, 1] below 8 (the default quintic: 1.21).
+ * rows, cols <= 2^20, rows * cols < 2^31, batch < 2^22 of the smallest matrices (a launch has less than 2^32 threads; else PWR_EUNSUPPORTED).
+ * Between the products entries end below 16: every iterate s of a singular value in [0, 1] that goes into a step has to keep s^2, |b s^2 + c s^4| and
+ * |a + b s^2 + c s^4| below 15.9 (the usual quintic: 1.5, 2.8, 3.5).  pwr_orthogonalize_range says whether coefficients do: 0, or PWR_EUNSUPPORTED, which
+ * is also what this call and pwr_muon_step return for those that do not.
  * ------------------------------------------------------------------------------------------- */
+int pwr_orthogonalize_range(int steps, float a, float b, float c);
 size_t pwr_orthogonalize_workspace_bytes(int rows, int cols, long long batch);
 int pwr_orthogonalize(const void* x, long long x_batch_stride, long long x_row_stride, void* out, int rows, int cols, long long batch, int dtype,
                       int steps, float a, float b, float c, float eps, void* workspace, size_t workspace_bytes, void* stream);

@@ -5,8 +5,8 @@
 // five steps bring everything above ~1e-3 of the norm into about 0.7 .. 1.2, i.e. X is near the closest orthogonal matrix U V^T.  A matrix with
 // more rows than columns is worked on transposed, so A and B are as small as they can be: m x m with m = min(rows, cols), n = max.
 //
-// Numbers.  Everything between the products is kept as a PAIR of fp16, hi + lo = 22 bits, scaled by 4096 (|X| <= ~1.2, |A| <= ~1.5, |B| <= ~4:
-// nothing overflows, and the low halves of entries down to 1e-5 are still normal fp16).  The matrix cores multiply fp16 pairs exactly and add in fp32.
+// Numbers.  Everything between the products is kept as a PAIR of fp16, hi + lo = 22 bits, scaled by 4096 (|X| <= ~1.2, |A| <= ~1.5, |B| <= ~4
+// with the coefficients above; others are refused where an entry could reach 16, the end of fp16, and the low halves of entries down to 1e-5 are still normal fp16).  The matrix cores multiply fp16 pairs exactly and add in fp32.
 //   fp32 tensors:  hi hi + hi lo + lo hi  -- three products per product; what is left out is 2^-22 of an entry, as much as an fp32 sum of this
 //                  length loses anyway (1e-6 of the result on the sizes tested, the same as fp32 products).
 //   bf16 tensors:  hi hi only -- one product -- but X itself advances from its 22 bits (the a X term), because noise put into X is amplified
@@ -20,6 +20,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <vector>
 
@@ -1203,6 +1204,32 @@ constexpr int kOrthMaxSide = 1 << 20;
 constexpr int kOrthMaxSteps = 64;
 constexpr long long kOrthMaxBlocks = 0xffffffffll / 1024;         // a launch has at most 2^32 - 1 threads
 
+// Every entry that is stored as a pair has to stay below 65504 / 4096 = 15.99.  The singular values of X0 fill [0, 1]; those of the next X are
+// s |a + b s^2 + c s^4|, and A, B and (in one workgroup) B + a I have s^2, b s^2 + c s^4 and a more than that.  A continuous odd map takes [-s, s] to
+// [-m, m], so the largest ones are followed exactly (0.2 % a step are left for the roundings); the last X is not stored.
+constexpr double kOrthLargest = 15.9;
+static double orth_quadratic(double k, double b, double c, double u) {         // max |k + b t + c t^2| over 0 <= t <= u
+  double m = std::max(fabs(k), fabs(k + u * (b + c * u)));
+  const double t = c != 0.0 ? -b / (2 * c) : -1.0;
+  return t > 0.0 && t < u ? std::max(m, fabs(k + t * (b + c * t))) : m;
+}
+static bool orth_range_ok(int steps, double a, double b, double c) {
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+  double s = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    const double u = s * s;
+    if (!(u < kOrthLargest) || !(orth_quadratic(0.0, b, c, u) < kOrthLargest) || !(orth_quadratic(a, b, c, u) < kOrthLargest)) return false;
+    auto next = [&](double t) { return sqrt(t) * fabs(a + t * (b + c * t)); };
+    double m = next(u);
+    // where the map turns: a + 3 b t + 5 c t^2 = 0
+    const double disc = 9 * b * b - 20 * a * c, root = disc > 0.0 ? sqrt(disc) : 0.0;
+    for (const double t : {c != 0.0 ? (-3 * b + root) / (10 * c) : b != 0.0 ? -a / (3 * b) : -1.0, c != 0.0 ? (-3 * b - root) / (10 * c) : -1.0})
+      if (disc >= 0.0 && t > 0.0 && t < u) m = std::max(m, next(t));
+    s = 1.002 * m;
+  }
+  return true;
+}
+
 static bool orth_shape_ok(long long rows, long long cols) {
   // (a matrix of up to 2^31 entries: tile counts and the entries of a plane's row stay in 32 bits, offsets are 64)
   return rows >= 1 && cols >= 1 && rows <= kOrthMaxSide && cols <= kOrthMaxSide && rows * cols <= 0x7fffffffll;
@@ -1211,6 +1238,11 @@ static bool orth_shape_ok(long long rows, long long cols) {
 }  // namespace pwr
 
 using namespace pwr;
+
+extern "C" int pwr_orthogonalize_range(int steps, float a, float b, float c) {
+  if (steps < 1 || steps > kOrthMaxSteps) return PWR_EINVAL;
+  return orth_range_ok(steps, a, b, c) ? 0 : PWR_EUNSUPPORTED;
+}
 
 extern "C" size_t pwr_orthogonalize_workspace_bytes(int rows, int cols, long long batch) {
   if (batch <= 0 || !orth_shape_ok(rows, cols)) return 0;
@@ -1265,6 +1297,7 @@ extern "C" int pwr_orthogonalize(const void* x, long long x_batch_stride, long l
   if (!x || !out || batch < 0 || x_batch_stride < 0 || x_row_stride < 0 || steps < 1 || steps > kOrthMaxSteps || !(eps >= 0.f)) return PWR_EINVAL;
   if (dtype != PWR_F32 && dtype != PWR_BF16) return PWR_EINVAL;
   if (!orth_shape_ok(rows, cols)) return rows < 1 || cols < 1 ? PWR_EINVAL : PWR_EUNSUPPORTED;
+  if (!orth_range_ok(steps, a, b, c)) return PWR_EUNSUPPORTED;
   if (!workspace || workspace_bytes < pwr_orthogonalize_workspace_bytes(rows, cols, batch)) return PWR_ENOSPACE;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == PWR_F32) return orthogonalize<float, 3>(x, x_batch_stride, x_row_stride, out, rows, cols, batch, steps, a, b, c, eps, workspace, s);
@@ -1444,6 +1477,7 @@ extern "C" int pwr_muon_step(const void* plan_host, const void* plan_dev, float*
   const MuonHead* h = (const MuonHead*)plan_host;
   if (!h || h->magic != kMuonMagic || !plan_dev || !p || !g || !buf || (h->rest && !v)) return PWR_EINVAL;
   if (ns_steps < 1 || ns_steps > kOrthMaxSteps || !(eps >= 0.f) || step < 1) return PWR_EINVAL;
+  if (h->items && !orth_range_ok(ns_steps, a, b, c)) return PWR_EUNSUPPORTED;
   if (h->items && (!workspace || workspace_bytes < h->ws_bytes)) return PWR_ENOSPACE;
   hipStream_t s = (hipStream_t)stream;
   const char* d = (const char*)plan_dev;

@@ -308,10 +308,17 @@ def _overlap(s, t):
     return s.numel() > 0 and t.numel() > 0 and s.device == t.device and a < d and c < b
 
 
+def _check_range(steps, a, b, c):
+    if _lib.lib().pwr_orthogonalize_range(steps, a, b, c) != 0:
+        raise ValueError("coefficients (%g, %g, %g): in %d steps some matrix reaches entries of 16 and more, which the products cannot hold" % (a, b, c, steps))
+
+
 def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
     """The matrices ``x`` (``[..., rows, cols]``, float32 or bfloat16) made nearly orthogonal by ``steps`` Newton-Schulz products:
     ``X = x / (|x| + eps)``, then ``X = a X + (b A + c A A) X`` with ``A = X X^T`` (of the shorter side).  With the default coefficients every singular
     value above about 1e-3 of the norm ends up between 0.7 and 1.2.  Float32: the precision of float32 products; bfloat16: 2e-3 of the result.
+
+    Other coefficients are taken as far as no entry of X, A or ``b A + c A A`` can reach 16 (``a I`` included): ValueError where some matrix would.
 
     Not differentiable (it is what an optimizer does to a gradient): a tensor that requires a gradient is refused."""
     _require_cuda(x, out)
@@ -324,6 +331,7 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
     steps = int(steps)
     if not 1 <= steps <= 64 or not float(eps) >= 0.0:
         raise ValueError("steps must be 1 .. 64 and eps not negative, got %d, %g" % (steps, eps))
+    _check_range(steps, a, b, c)
     rows, cols = x.shape[-2:]
     if x.numel() and (max(rows, cols) > 2 ** 20 or rows * cols > _INT):      # (before they cross the C ABI as int, which would cut them)
         raise ValueError("matrices of %d x %d are larger than orthogonalize takes (2^20 a side, 2^31 - 1 entries)" % (rows, cols))

@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import NS_COEFFICIENTS, _on
+from .ops import NS_COEFFICIENTS, _check_range, _on
 
 
 class _Param(ctypes.Structure):
@@ -36,10 +36,11 @@ class Muon:
         self._check(flat, "flat")
         if not 1 <= int(ns_steps) <= 64 or not float(eps) >= 0.0:
             raise ValueError("ns_steps must be 1 .. 64 and eps not negative, got %d, %g" % (ns_steps, eps))
-        if len(tuple(coefficients)) != 3:
+        coefficients = tuple(float(c) for c in coefficients)
+        if len(coefficients) != 3:
             raise ValueError("coefficients are (a, b, c)")
         self.lr, self.momentum, self.nesterov, self.weight_decay, self.update_rms = lr, momentum, nesterov, weight_decay, update_rms
-        self.ns_steps, self.coefficients, self.eps = int(ns_steps), tuple(float(c) for c in coefficients), eps
+        self.ns_steps, self.coefficients, self.eps = int(ns_steps), coefficients, eps
         self.beta1, self.beta2, self.adam_eps = beta1, beta2, adam_eps
         self.buf = torch.zeros_like(flat) if buf is None else self._check(buf, "buf")
         self.v = torch.zeros_like(flat) if v is None else self._check(v, "v")
@@ -52,6 +53,8 @@ class Muon:
                     raise ValueError("a parameter of %d elements (2^31 at most)" % n)
                 params.append((at, rows, n // rows))
             at += n
+        if any(min(rows, cols) > 1 for _, rows, cols in params):
+            _check_range(self.ns_steps, *self.coefficients)
         self._plan = self._ws = None
         if not params:
             return

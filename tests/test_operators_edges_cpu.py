@@ -1,8 +1,13 @@
 """CPU: calls at the edge of what log_likelihood, orthogonalize and Muon take."""
+import ctypes
+import math
+
+import numpy as np
 import pytest
 import torch
 
-from pixelwiseregression_amd import _lib, ops
+from pixelwiseregression_amd import _lib, ops, optim
+from pixelwiseregression_amd.optim import _Param
 
 EUNSUPPORTED = -2
 SOME = 4096        # an address that is never read: every call below is refused on the host
@@ -60,3 +65,60 @@ def test_numbers_of_rows_whose_launch_leaves_64_bits_are_refused():
     for rows in (2 ** 32, 2 ** 58, 2 ** 62):
         for V in (4, 600, 40000):
             assert forward(rows, V, 0) == EUNSUPPORTED and forward(rows, V, 0, 1) == EUNSUPPORTED and backward(rows, V, 0) == EUNSUPPORTED
+
+
+def largest(steps, a, b, c, n=20001):
+    """The largest entry that could be stored: max of s, s^2, |b s^2 + c s^4| and |a + b s^2 + c s^4| over the iterates of [0, 1] that go into a step."""
+    s, m = np.linspace(0, 1, n), 0.0
+    with np.errstate(over="ignore", invalid="ignore"):
+        for _ in range(steps):
+            u = s * s
+            q = b * u + c * u * u
+            m = max(m, u.max(), np.abs(q).max(), np.abs(a + q).max())
+            if not m < 1e3:
+                return math.inf
+            s = np.linspace(0, np.abs(s * (a + q)).max(), n)
+    return m
+
+
+def test_coefficients_that_leave_the_pairs_are_refused(anywhere):
+    l = _lib.lib()
+    r = np.random.default_rng(0)
+    taken = refused = 0
+    for _ in range(400):
+        steps = int(r.integers(1, 9))
+        co = [float(np.float32(v)) for v in (r.uniform(-4, 4), r.uniform(-8, 8) * r.choice([0, 1]), r.uniform(-4, 4) * r.choice([0, 1]))]
+        m, got = largest(steps, *co), l.pwr_orthogonalize_range(steps, *co)
+        if m > 16.0:
+            assert got == EUNSUPPORTED, (steps, co, m)
+            refused += 1
+        elif m < 15.9 / 1.002 ** (4 * steps) / 1.1:               # (away from the border, where an unstable map makes much of the room for roundings)
+            taken += got == 0
+            assert got == 0 or largest(steps, *[1.01 * v for v in co]) > 15.9, (steps, co, m)
+    assert taken > 50 and refused > 50
+    for steps in (1, 2, 5, 64):
+        for co in (ops.NS_COEFFICIENTS, (1.5, -0.5, 0.0), (15 / 8, -10 / 8, 3 / 8), (2.0, -1.5, 0.5)):
+            assert l.pwr_orthogonalize_range(steps, *co) == 0
+    # linear maps and single steps: both sides of each limit
+    for steps, co, ok in ((3, (1.98, 0.0, 0.0), 1), (3, (2.0, 0.0, 0.0), 0), (1, (1.0, -15.8, 0.0), 1), (1, (1.0, -16.0, 0.0), 0), (1, (15.8, -15.8, 0.0), 1),
+                          (1, (16.0, -15.0, 0.0), 0), (2, (2.5, -0.06, 0.0), 1), (4, (2.5, -0.06, 0.0), 0), (5, (3.0, -0.065, 0.0), 0),
+                          (1, (math.nan, 0.0, 0.0), 0), (1, (0.0, math.inf, 0.0), 0)):
+        assert (l.pwr_orthogonalize_range(steps, *co) == 0) == bool(ok), (steps, co)
+        if not ok:
+            assert l.pwr_orthogonalize(SOME, 12, 4, SOME, 3, 4, 1, 0, steps, *co, 1e-7, SOME, 2 ** 40, None) == EUNSUPPORTED
+            with pytest.raises(ValueError, match="coefficients"):
+                ops.orthogonalize(empty(3, 4), steps=steps, coefficients=co)
+    assert l.pwr_orthogonalize_range(0, 1.5, -0.5, 0.0) == -1 and l.pwr_orthogonalize_range(65, 1.5, -0.5, 0.0) == -1
+
+
+def test_the_optimizer_refuses_such_coefficients(monkeypatch):
+    l = _lib.lib()
+    monkeypatch.setattr(optim.Muon, "_check", lambda self, t, what: t)
+    with pytest.raises(ValueError, match="coefficients"):
+        optim.Muon(torch.zeros(20), [(4, 5)], coefficients=(3.0, -0.065, 0.0))
+    arr = (_Param * 1)((0, 4, 5))
+    n = l.pwr_muon_plan_bytes(arr, 1)
+    plan = ctypes.create_string_buffer(n)
+    assert l.pwr_muon_plan(arr, 1, plan) == 0
+    step = lambda ns, *co: l.pwr_muon_step(plan, SOME, SOME, SOME, SOME, SOME, 1e-3, .95, 1, 0., .2, ns, *co, 1e-7, .9, .999, 1e-8, 1, 1., SOME, 2 ** 40, None)  # noqa: E731
+    assert step(5, 3.0, -0.065, 0.0) == EUNSUPPORTED and step(1, 1.0, -16.0, 0.0) == EUNSUPPORTED
