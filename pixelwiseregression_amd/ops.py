@@ -5,6 +5,7 @@ Only device tensors are accepted: there is no CPU implementation behind these op
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -110,6 +111,11 @@ def _dtype_tag(t, what):
     if t.dtype not in _DTYPES:
         raise ValueError("%s must be float32 or bfloat16, got %s" % (what, t.dtype))
     return _DTYPES[t.dtype]
+
+
+def _tangents(*ts):
+    """Whether one of them carries a forward-mode tangent (requires_grad says nothing of those)."""
+    return forward_ad._current_level >= 0 and any(t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _same_device(t, *others):
@@ -262,12 +268,15 @@ def log_likelihood(z, index, w=None, mask=None, topk=0):
     (one per sample) or one per map; 0 = not allowed, whatever z holds there.  topk <= 32 (less for maps of over 2^21 pixels): equal values go by the lowest index; what does not exist
     (masked, -inf, beyond the map) is ``(-inf, -1)``.  A map without an allowed pixel: -inf, entropy 0, zero gradient.
 
-    Returns ``LogLikelihood(logp, entropy, top_logp, top_index)``, float32 (int64 the last); gradients of ``logp`` and ``entropy`` reach z and w.
+    Returns ``LogLikelihood(logp, entropy, top_logp, top_index)``, float32 (int64 the last); gradients of ``logp`` and ``entropy`` reach z and w
+    (reverse mode; a forward-mode tangent is refused).
     In a captured graph: ``likelihood_gradients``, or forward and backward with no other autograd graph of the same leaves alive."""
     _require_cuda(z, index, w, mask)
     topk = int(topk)
     if not 0 <= topk <= 32:
         raise ValueError("topk must be 0 .. 32, got %d" % topk)
+    if _tangents(z, w):
+        raise NotImplementedError("log_likelihood has no forward-mode derivative")
     if torch.is_grad_enabled() and (z.requires_grad or (w is not None and w.requires_grad)):
         return LogLikelihood(*LogLikelihoodFn.apply(z, w, index, mask, topk))
     return LogLikelihood(*_likelihood_forward(_Rows(z, index, w, mask), topk, False)[:4])
@@ -277,6 +286,8 @@ def likelihood_gradients(z, index, w, glogp, gentropy, mask=None):
     """``log_likelihood(z, index, w, mask)`` and, without an autograd graph, the gradients of ``sum(glogp logp) + sum(gentropy entropy)`` with
     respect to z and w (float32 ``[J]``).  Returns ``(LogLikelihood, gz, gw)``; gw is None without w."""
     _require_cuda(z, index, w, glogp, gentropy, mask)
+    if _tangents(z, w, glogp, gentropy):
+        raise NotImplementedError("likelihood_gradients has no forward-mode derivative")
     with torch.no_grad():
         r = _Rows(z, index, w, mask)
         for g in (glogp, gentropy):
@@ -320,12 +331,12 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
 
     Other coefficients are taken as far as no entry of X, A or ``b A + c A A`` can reach 16 (``a I`` included): ValueError where some matrix would.
 
-    Not differentiable (it is what an optimizer does to a gradient): a tensor that requires a gradient is refused."""
+    Not differentiable (it is what an optimizer does to a gradient): a tensor that requires a gradient, or carries a forward-mode tangent, is refused."""
     _require_cuda(x, out)
     tag = _dtype_tag(x, "x")
     if x.dim() < 2:
         raise ValueError("x must be a matrix or a batch of them, got %s" % (tuple(x.shape),))
-    if torch.is_grad_enabled() and x.requires_grad:
+    if (torch.is_grad_enabled() and x.requires_grad) or _tangents(x, out):
         raise NotImplementedError("orthogonalize has no gradient: detach x")
     a, b, c = (float(t) for t in coefficients)
     steps = int(steps)

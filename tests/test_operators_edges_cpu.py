@@ -122,3 +122,20 @@ def test_the_optimizer_refuses_such_coefficients(monkeypatch):
     assert l.pwr_muon_plan(arr, 1, plan) == 0
     step = lambda ns, *co: l.pwr_muon_step(plan, SOME, SOME, SOME, SOME, SOME, 1e-3, .95, 1, 0., .2, ns, *co, 1e-7, .9, .999, 1e-8, 1, 1., SOME, 2 ** 40, None)  # noqa: E731
     assert step(5, 3.0, -0.065, 0.0) == EUNSUPPORTED and step(1, 1.0, -16.0, 0.0) == EUNSUPPORTED
+
+
+def test_forward_mode_tangents_are_refused(anywhere):
+    """(no requires_grad on a dual tensor: its derivative would be dropped without a word)"""
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        z, w = (fw.make_dual(t, torch.ones_like(t)) for t in (torch.zeros(2, 3, 8), torch.ones(3)))
+        assert not z.requires_grad and not w.requires_grad
+        for call in (lambda: ops.log_likelihood(z, None), lambda: ops.log_likelihood(torch.zeros(2, 3, 8), None, w),
+                     lambda: ops.likelihood_gradients(z, None, None, None, None), lambda: ops.likelihood_gradients(torch.zeros(2, 3, 8), None, w, None, None),
+                     lambda: ops.orthogonalize(z)):
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+        assert not ops._tangents(torch.zeros(3), None)
+    assert not ops._tangents(z, w)
