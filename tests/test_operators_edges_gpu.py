@@ -35,3 +35,37 @@ def test_coefficients_at_the_end_of_the_range(rows, cols, dtype, steps, co):
         out = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
         assert np.isfinite(got).all()
         assert np.linalg.norm(got - ref) <= noise + out * np.linalg.norm(ref), (kind, np.linalg.norm(got - ref), noise, np.linalg.norm(ref))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_results_can_be_changed_in_place(grad):
+    """The -inf of an empty map cleared, a sign turned, one entry set: without an error, in this result alone, and the gradient is that of the rest."""
+    from pixelwiseregression_amd import ops
+    z = torch.randn(4, 3, 50, device=DEV)
+    mask = torch.ones(4, 1, 50, device=DEV)
+    mask[1] = 0
+    index = torch.randint(0, 50, (4, 3), device=DEV)
+    a, b = (z.clone().requires_grad_(grad) for _ in range(2))
+    r, q = ops.log_likelihood(a, index, None, mask), ops.log_likelihood(b, index, None, mask)
+    entropy = q.entropy.clone()
+    empty = torch.isinf(r.logp)
+    assert empty[1].all() and empty.sum() == 3
+    changed = r.logp.masked_fill_(empty, 0.0)
+    r.logp.neg_()
+    r.logp[0, 0] = 7.0
+    assert r.logp[0, 0] == 7.0 and (r.logp[1] == 0).all() and torch.equal(r.entropy, entropy) and r.entropy._version == 0
+    keep = ~empty
+    keep[0, 0] = False
+    assert torch.equal(r.logp[keep], -q.logp[keep])
+    assert r.logp.untyped_storage().data_ptr() != r.entropy.untyped_storage().data_ptr()
+    if not grad:
+        scale = torch.ones(4, 3, device=DEV, requires_grad=True)
+        assert r.logp.mul_(scale).requires_grad
+        return
+    (ga,) = torch.autograd.grad(changed.sum() + r.entropy.sum(), a)
+    (gb,) = torch.autograd.grad(torch.where(keep, -q.logp, torch.zeros_like(q.logp)).sum() + q.entropy.sum(), b)
+    assert torch.equal(ga, gb)
+    fresh = ops.log_likelihood(a, index)
+    fresh.entropy.neg_()                                      # (what the gradient needs: noticed)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(fresh.logp.sum(), a)
