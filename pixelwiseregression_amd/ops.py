@@ -323,6 +323,11 @@ def _check_range(steps, a, b, c):
         raise ValueError("coefficients (%g, %g, %g): in %d steps some matrix reaches entries of 16 and more, which the products cannot hold" % (a, b, c, steps))
 
 
+def _written(*ts):
+    """A kernel has written to them: a gradient that saved one before notices, as after an in-place operation."""
+    torch.autograd.graph.increment_version([t for t in ts if not t.is_inference()])
+
+
 def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
     """The matrices ``x`` (``[..., rows, cols]``, float32 or bfloat16) made nearly orthogonal by ``steps`` Newton-Schulz products:
     ``X = x / (|x| + eps)``, then ``X = a X + (b A + c A A) X`` with ``A = X X^T`` (of the shorter side).  With the default coefficients every singular
@@ -345,8 +350,11 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
     rows, cols = x.shape[-2:]
     if x.numel() and (max(rows, cols) > 2 ** 20 or rows * cols > _INT):      # (before they cross the C ABI as int, which would cut them)
         raise ValueError("matrices of %d x %d are larger than orthogonalize takes (2^20 a side, 2^31 - 1 entries)" % (rows, cols))
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    elif torch.is_grad_enabled() and out.requires_grad:
+        raise NotImplementedError("orthogonalize has no gradient: detach out")
     elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous %s tensor of shape %s" % (x.dtype, tuple(x.shape)))
     elif _overlap(x, out) and not (out.data_ptr() == x.data_ptr() and x.is_contiguous()):
@@ -363,4 +371,6 @@ def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
     with _on(x.device):
         _lib.check(l.pwr_orthogonalize(v.data_ptr(), v.stride(0), v.stride(1), out.data_ptr(), rows, cols, v.shape[0], tag, steps, a, b, c, float(eps),
                                        ws.data_ptr(), need, _lib.stream_ptr(x.device)), "pwr_orthogonalize")
+    if given:
+        _written(out)
     return out

@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import NS_COEFFICIENTS, _check_range, _on
+from .ops import NS_COEFFICIENTS, _check_range, _on, _written
 
 
 class _Param(ctypes.Structure):
@@ -91,6 +91,7 @@ class Muon:
                 self._plan, self._plan_dev.data_ptr(), self.flat.data_ptr(), grad.data_ptr(), self.buf.data_ptr(), self.v.data_ptr(), self.lr,
                 self.momentum, 1 if self.nesterov else 0, self.weight_decay, self.update_rms, self.ns_steps, a, b, c, self.eps, self.beta1, self.beta2,
                 self.adam_eps, self.steps, grad_scale, self._ws.data_ptr(), self._ws.numel(), _lib.stream_ptr(self.flat.device)), "pwr_muon_step")
+        _written(self.flat, self.buf, self.v)
 
     def state_dict(self):
         return {"buf": self.buf.clone(), "v": self.v.clone(), "steps": self.steps}

@@ -69,3 +69,24 @@ def test_results_can_be_changed_in_place(grad):
     fresh.entropy.neg_()                                      # (what the gradient needs: noticed)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(fresh.logp.sum(), a)
+
+
+def test_what_is_written_counts_as_changed():
+    """A gradient that saved a tensor before orthogonalize(out=) or a Muon step wrote to it notices."""
+    from pixelwiseregression_amd import ops, optim
+    w = torch.ones(8, 9, device=DEV, requires_grad=True)
+    for write in (lambda t: ops.orthogonalize(t, out=t), lambda t: ops.orthogonalize(torch.randn(8, 9, device=DEV), out=t),
+                  lambda t: optim.Muon(t.view(-1), [(8, 9)]).step(torch.randn(72, device=DEV))):
+        x = torch.randn(8, 9, device=DEV)
+        y = (w * x).sum()
+        write(x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        x = torch.randn(8, 9, device=DEV)
+        assert ops.orthogonalize(x, out=x) is x
+        optim.Muon(x.view(-1), [(8, 9)]).step(x.clone().view(-1))
+    with pytest.raises(NotImplementedError):
+        ops.orthogonalize(torch.randn(8, 9, device=DEV), out=w)
+    with torch.no_grad():
+        assert ops.orthogonalize(torch.randn(8, 9, device=DEV), out=w) is w
