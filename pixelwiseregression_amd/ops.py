@@ -182,6 +182,8 @@ class _Rows:
         self.mask_rows = 1
         self.mask = mask
         if mask is not None:
+            if dim == 4 and mask.dim() == 4 and mask.shape[2:] != shape[2:]:       # (as many pixels in other rows are no mask of these)
+                raise ValueError("mask must be %s a map, got %s" % (tuple(shape[2:]), tuple(mask.shape)))
             m = mask.flatten(2) if dim == 4 and mask.dim() == 4 else mask
             if dim > 2 and m.shape == (lead[0], 1, self.V):
                 self.mask_rows = J

@@ -139,3 +139,14 @@ def test_forward_mode_tangents_are_refused(anywhere):
                 call()
         assert not ops._tangents(torch.zeros(3), None)
     assert not ops._tangents(z, w)
+
+
+def test_a_mask_is_of_the_maps_own_shape():
+    z = torch.zeros(2, 3, 4, 6)
+    with pytest.raises(ValueError, match="mask"):
+        ops._Rows(z, None, None, torch.ones(2, 1, 6, 4))
+    with pytest.raises(ValueError, match="mask"):
+        ops._Rows(z, None, None, torch.ones(2, 3, 2, 12))
+    for m in (torch.ones(2, 1, 4, 6), torch.ones(2, 3, 4, 6), torch.ones(2, 1, 24), torch.ones(2, 3, 24)):
+        r = ops._Rows(z, None, None, m)
+        assert r.mask.shape == m.flatten(2).shape and r.mask_rows == (3 if m.shape[1] == 1 else 1)
