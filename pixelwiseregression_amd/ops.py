@@ -185,6 +185,8 @@ class _Rows:
             if dim == 4 and mask.dim() == 4 and mask.shape[2:] != shape[2:]:       # (as many pixels in other rows are no mask of these)
                 raise ValueError("mask must be %s a map, got %s" % (tuple(shape[2:]), tuple(mask.shape)))
             m = mask.flatten(2) if dim == 4 and mask.dim() == 4 else mask
+            if m.dtype is torch.float64:
+                m = m != 0                                                         # (what float32 would round to 0 is allowed)
             if dim > 2 and m.shape == (lead[0], 1, self.V):
                 self.mask_rows = J
             elif m.shape != lead + (self.V,):

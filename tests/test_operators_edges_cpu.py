@@ -150,3 +150,13 @@ def test_a_mask_is_of_the_maps_own_shape():
     for m in (torch.ones(2, 1, 4, 6), torch.ones(2, 3, 4, 6), torch.ones(2, 1, 24), torch.ones(2, 3, 24)):
         r = ops._Rows(z, None, None, m)
         assert r.mask.shape == m.flatten(2).shape and r.mask_rows == (3 if m.shape[1] == 1 else 1)
+
+
+def test_a_mask_of_any_type_keeps_what_is_not_zero():
+    values = [0.0, 1.0, 1e-300, -0.0, 5e-324, math.nan, 1e300]
+    want = [False, True, True, False, True, True, True]
+    r = ops._Rows(torch.zeros(1, 7), None, None, torch.tensor([values], dtype=torch.float64))
+    assert r.mask.dtype is torch.float32 and (r.mask[0] != 0).tolist() == want
+    for dtype in (torch.bool, torch.uint8, torch.int64, torch.float16, torch.bfloat16, torch.float32):
+        m = torch.tensor([[0, 1, 1, 0, 1, 1, 1]]).to(dtype)
+        assert (ops._Rows(torch.zeros(1, 7), None, None, m).mask[0] != 0).tolist() == want
