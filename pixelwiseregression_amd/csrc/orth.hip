@@ -853,7 +853,8 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
   __shared__ double red[8];
   int t; int4 tile;
   const OrthItem o = orth_item(g, blockIdx.x, t, tile);
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, li = lane & 15, lg = lane >> 4;
+  // (the wave's number as a scalar: branches on it are jumps; as a lane's value the phases of A below spill three registers)
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, lg = lane >> 4;
   const bool tall = o.rows > o.cols;
   const int m = tall ? o.cols : o.rows, n = tall ? o.rows : o.cols;
   const int NP = (n + 63) & ~63;                        // <= NCAP
@@ -941,12 +942,20 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
     *reinterpret_cast<half4*>(at) = h;
     *reinterpret_cast<half4*>(at + plane) = l;
   };
-  auto gram = [&](auto half) {
+  // A, in phases between the workgroup's barriers: the waves of a pair have tiles of their own, the barriers are everyone's
+  constexpr int MOST = Tri::n[0] > Tri::n[1] ? Tri::n[0] : Tri::n[1];
+  f32x4 sums[MOST];
+  const int quarter = wid >> 1;
+  auto halves = [&](auto&& phase) {
+    if (wid & 1) phase(std::integral_constant<int, 1>{});
+    else phase(std::integral_constant<int, 0>{});
+  };
+  // tile k is finished by the wave of quarter k & 3: the other three leave it their sums
+  auto slot = [&](int h, int u, int k) { return reinterpret_cast<f32x4*>(R + ((u * TRI + h * Tri::n[0] + k) * 64 + lane) * 16); };
+  auto gram_sums = [&](auto half) {
     constexpr int H = decltype(half)::value, NT = Tri::n[H];
-    const int quarter = wid >> 1;
-    f32x4 acc[NT];
 #pragma unroll
-    for (int k = 0; k < NT; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < NT; ++k) sums[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int ks = quarter; ks < NP / 32; ks += 4) {
       half8 f[MT][2];
 #pragma unroll
@@ -954,20 +963,22 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
 #pragma unroll
         for (int p = 0; p < 2; ++p) f[r][p] = *reinterpret_cast<const half8*>(X + p * xplane + xat(16 * r + li, ks * 4 + lg));
 #pragma unroll
-      for (int k = 0; k < NT; ++k) acc[k] = mfma4(f[Tri::p[H][k]], f[Tri::q[H][k]], acc[k]);
+      for (int k = 0; k < NT; ++k) sums[k] = mfma4(f[Tri::p[H][k]], f[Tri::q[H][k]], sums[k]);
     }
-    // tile k is finished by the wave of quarter k & 3: the other three leave it their sums
-    auto slot = [&](int u, int k) { return reinterpret_cast<f32x4*>(R + ((u * TRI + H * Tri::n[0] + k) * 64 + lane) * 16); };
 #pragma unroll
     for (int k = 0; k < NT; ++k)
-      if ((k & 3) != quarter) *slot((quarter - k - 1) & 3, k) = acc[k];
-    __syncthreads();
+      if ((k & 3) != quarter) *slot(H, (quarter - k - 1) & 3, k) = sums[k];
+  };
+  auto gram_add = [&](auto half) {
+    constexpr int H = decltype(half)::value, NT = Tri::n[H];
 #pragma unroll
     for (int k = 0; k < NT; ++k)
       if ((k & 3) == quarter)
 #pragma unroll
-        for (int u = 0; u < 3; ++u) acc[k] += *slot(u, k);
-    __syncthreads();
+        for (int u = 0; u < 3; ++u) sums[k] += *slot(H, u, k);
+  };
+  auto gram_put = [&](auto half) {
+    constexpr int H = decltype(half)::value, NT = Tri::n[H];
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
       if ((k & 3) != quarter) continue;
@@ -975,7 +986,7 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
       float v[4];
       half4 h, l;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = acc[k][e] * (kOrthInv * kOrthInv);
+      for (int e = 0; e < 4; ++e) v[e] = sums[k][e] * (kOrthInv * kOrthInv);
       put4(R + aat(i, j >> 3) + (j & 7) * 2, aplane, v, h, l);
       if (Tri::p[H][k] != Tri::q[H][k]) {
 #pragma unroll
@@ -986,11 +997,14 @@ __global__ __launch_bounds__(512) void orth_small_kernel(OrthArgs g, SRC src, OU
         }
       }
     }
-    __syncthreads();
   };
   for (int step = 0; step < steps; ++step) {
-    if (wid & 1) gram(std::integral_constant<int, 1>{});
-    else gram(std::integral_constant<int, 0>{});
+    halves(gram_sums);
+    __syncthreads();
+    halves(gram_add);
+    __syncthreads();
+    halves(gram_put);
+    __syncthreads();
     // B + a I
     constexpr int PW = MT == 4 ? 2 : 1;
     const int q = MT == 4 ? wid >> 1 : (wid >> 1) & 1, p0 = MT == 4 ? 2 * (wid & 1) : wid & 1;

@@ -160,3 +160,30 @@ def test_a_mask_of_any_type_keeps_what_is_not_zero():
     for dtype in (torch.bool, torch.uint8, torch.int64, torch.float16, torch.bfloat16, torch.float32):
         m = torch.tensor([[0, 1, 1, 0, 1, 1, 1]]).to(dtype)
         assert (ops._Rows(torch.zeros(1, 7), None, None, m).mask[0] != 0).tolist() == want
+
+
+def test_the_barriers_of_one_workgroup_are_every_waves():
+    """In the kernel of small matrices the waves of a pair take different branches: none of its barriers stands inside one, or inside a function that is
+    called from one."""
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(root, "pixelwiseregression_amd", "csrc", "orth.hip")).read())
+    text = text[text.index("void orth_small_kernel("):]
+    stack, head, barriers = [], "", 0
+    for token in re.split(r"([{};])", text):
+        if token == "{":
+            stack.append(head)
+        elif token == "}":
+            stack.pop()
+            if not stack:
+                break
+        elif token != ";":
+            if "__syncthreads" in token:
+                barriers += 1
+                assert "if (" not in token and not any("[&]" in h or "if (" in h for h in stack[1:]), stack[1:]
+        if token in "{};":
+            head = ""
+        else:
+            head = token
+    assert barriers >= 7
