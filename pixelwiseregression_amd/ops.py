@@ -207,7 +207,7 @@ def _likelihood_forward(r, topk, stats):
     z, dev, lead = r.z, r.z.device, r.lead
     # (each result its own tensor: views of one buffer could not be changed in place, and would share a version)
     logp = torch.empty(lead, device=dev, dtype=torch.float32) if r.index is not None else None
-    entropy = torch.empty(lead, device=dev, dtype=torch.float32)
+    entropy = torch.empty(lead, device=dev, dtype=torch.float32) if logp is None else torch.empty_like(logp)
     top_logp = torch.empty(lead + (topk,), device=dev, dtype=torch.float32) if topk else None
     top_index = torch.empty(lead + (topk,), device=dev, dtype=torch.int64) if topk else None
     st = torch.empty((r.rows, 2), device=dev, dtype=torch.float32) if stats else None
