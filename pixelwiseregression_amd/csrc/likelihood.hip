@@ -321,7 +321,8 @@ __global__ __launch_bounds__(NT) void like_fwd_kernel(LikeArgs a) {
 }
 
 // Long rows, enough of them to fill the chip, without alternatives: one workgroup walks its row in parts of NT x VPT values, the next part's loads under
-// way while it works on one.  The sums are kept relative to the largest value so far, per thread; one barrier per part.  4096 rows of 50001 bf16: 256 threads
+// way while it works on one.  The sums are kept relative to the largest value so far, per thread; one barrier per part.  A part's sixteen values are added up
+// by themselves and the parts by compensated additions: the length of the row costs no bits, a new maximum one rounding.  4096 rows of 50001 bf16: 256 threads
 // x 16 values 102 us = 4.0 TB/s (50000, rows that start aligned: 88 us = 4.7), 256 x 32 112, 512 x 16 128, 1024 x 16 189, a workgroup per chunk and a
 // join 161; 5376 rows of 16384 fp32: 64 us = 5.5 TB/s against 74 in one piece.
 template <typename T, int NT, int VPT>
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(NT) void like_walk_kernel(LikeArgs a) {
   RowPart<T, NT, VPT> part;
   part.load(z, mrow, a.V);
   const LikeGiven given = like_given<T>(a, t, z, mrow, w);
-  float M = -INFINITY, c = 0.f, r = 0.f, q = 0.f;
+  float M = -INFINITY, c = 0.f, r = 0.f, q = 0.f, dr = 0.f, dq = 0.f;     // (what the last additions to r and q lost)
   for (int base = 0, turn = 0; base < a.V; base += PART, turn ^= 1) {
     const int n = a.V - base;
     float s[VPT], v[VPT];
@@ -353,9 +354,11 @@ __global__ __launch_bounds__(NT) void like_walk_kernel(LikeArgs a) {
 #pragma unroll
     for (int k = 0; k < NW; ++k) m = fmaxf(m, top[turn][k]);
     if (m > M) {
-      const LikeStat x = like_shift(LikeStat{M, c, r, q}, m);
+      const LikeStat x = like_shift(LikeStat{M, c, r - dr, q - dq}, m);
       c = x.c; r = x.r; q = x.q; M = m;
+      dr = dq = 0.f;
     }
+    float pr = 0.f, pq = 0.f;                                      // of this part
     const float m0 = M == -INFINITY ? 0.f : M;
     if (__any(own == m0 && M > -INFINITY)) {                        // a wave that has values at the maximum counts them
 #pragma unroll
@@ -363,8 +366,8 @@ __global__ __launch_bounds__(NT) void like_walk_kernel(LikeArgs a) {
         const float d = s[k] - m0, x = __expf(d);
         const bool at = d == 0.f;
         c += at ? 1.f : 0.f;
-        r += at ? 0.f : x;
-        q = fmaf(x, fmaxf(d, -1e30f), q);
+        pr += at ? 0.f : x;
+        pq = fmaf(x, fmaxf(d, -1e30f), pq);
       }
     } else {
 #pragma unroll
@@ -373,12 +376,16 @@ __global__ __launch_bounds__(NT) void like_walk_kernel(LikeArgs a) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           const float d = s[k * N + e] - m0, x = __expf(d);
-          r += x;
-          q = fmaf(x, fmaxf(d, -1e30f), q);
+          pr += x;
+          pq = fmaf(x, fmaxf(d, -1e30f), pq);
         }
       }
     }
+    const float yr = pr - dr, yq = pq - dq, nr = r + yr, nq = q + yq;
+    dr = (nr - r) - yr; dq = (nq - q) - yq;
+    r = nr; q = nq;
   }
+  r -= dr; q -= dq;
   c = wave_sum(c); r = wave_sum(r); q = wave_sum(q);
   if (lane == 0) { sum[0][wid] = c; sum[1][wid] = r; sum[2][wid] = q; }
   __syncthreads();

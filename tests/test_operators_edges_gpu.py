@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from oracle import muon_ref
+from oracle import likelihood_ref, muon_ref
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -90,3 +90,31 @@ def test_what_is_written_counts_as_changed():
         ops.orthogonalize(torch.randn(8, 9, device=DEV), out=w)
     with torch.no_grad():
         assert ops.orthogonalize(torch.randn(8, 9, device=DEV), out=w) is w
+
+
+@pytest.mark.parametrize("V", [50001, 131072, 1048579])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_walked_rows(V, dtype):
+    """Rows of unequal values that one workgroup walks (512 of them and more, no alternatives; here 600 that are one row in memory).  A thread adds sixteen
+    values at a time and those sums without loss, then come 2 + 6 + 3 additions: with the roundings of test_likelihood_gpu.py's tolerance for s, s - M
+    and the exponent at most 64 in a row, whatever the length.  A new maximum costs what is there three more (the factor's two and the product's); of
+    the rising row with a new one in each of V / 4096 parts, f = e^(-60 * 4096 / V) apart, f / (1 - f) <= 4 parts count: (4 S + 128 + 12) 2^-24."""
+    from pixelwiseregression_amd import ops
+    g = torch.Generator().manual_seed(V)
+    z = 3.0 * torch.randn(5, V, generator=g)
+    z[1] *= 0.01                                              # nearly uniform: every value counts
+    z[2] = torch.linspace(-30, 30, V)                         # a new maximum in every part
+    z[3] = torch.linspace(20, 0, V)                           # the maximum first
+    z[4] = -0.37                                              # equal terms, whose roundings are equal too: one after another, 2^20 of them lose 934 2^-24
+    z[4, 0] = 0.0
+    z = z.to(dtype)
+    index = torch.tensor([5, V - 1, V // 2, V // 3, 1])
+    ref = likelihood_ref.rows(z.float().numpy()[:, None], index.numpy()[:, None])
+    zd = z.to(DEV)
+    for k in range(5):
+        r = ops.log_likelihood(zd[k:k + 1].expand(600, V), index[k:k + 1].to(DEV).expand(600))
+        assert (r.logp == r.logp[0]).all() and (r.entropy == r.entropy[0]).all()
+        tol = (4 * z[k].float().abs().max().item() + 140) * 2.0 ** -24
+        lp, h = ref["logp"][k, 0], ref["entropy"][k, 0]
+        assert abs(r.logp[0].item() - lp) <= tol, (k, r.logp[0].item(), lp, tol)
+        assert abs(r.entropy[0].item() - h) <= (1 + h) * tol, (k, r.entropy[0].item(), h, tol)
