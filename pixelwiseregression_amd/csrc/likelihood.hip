@@ -619,14 +619,16 @@ __global__ __launch_bounds__(256) void like_bwd_wave_kernel(LikeBwdArgs a) {
   }
 }
 
-// gw[j] = the partial sums of the rows of joint j, in their order
+// gw[j] = the partial sums of the rows of joint j, in their order.  In 64 bits: a thread adds every 256th of them, thousands where the rows are many.
 __global__ __launch_bounds__(256) void like_gw_kernel(const float* __restrict__ part, float* __restrict__ gw, long long samples, int J, int chunks) {
-  __shared__ float red[4];
+  __shared__ double red[4];
   const int j = blockIdx.x;
-  float s = 0.f;
+  double s = 0.0;
   for (long long k = threadIdx.x; k < samples * chunks; k += 256) s += part[((k / chunks) * J + j) * chunks + k % chunks];
-  s = block_sum1(s, red);
-  if (threadIdx.x == 0) gw[j] = s;
+  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) gw[j] = (float)((red[0] + red[1]) + (red[2] + red[3]));
 }
 
 }  // namespace pwr

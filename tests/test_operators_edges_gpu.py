@@ -118,3 +118,16 @@ def test_long_walked_rows(V, dtype):
         lp, h = ref["logp"][k, 0], ref["entropy"][k, 0]
         assert abs(r.logp[0].item() - lp) <= tol, (k, r.logp[0].item(), lp, tol)
         assert abs(r.entropy[0].item() - h) <= (1 + h) * tol, (k, r.entropy[0].item(), h, tol)
+
+
+def test_the_gradient_of_w_over_many_rows():
+    """2^20 equal rows of two logits 0 and 1, the pixel at 0: dL/dw = -2^20 g p(1), each row off by what test_likelihood_gpu.py allows, 2 (4 S + 128) 2^-24 of
+    its terms g p(1) z; their sum loses nothing but its own rounding.  (One after another, 4096 a thread, equal terms lose 510 2^-24.)"""
+    from pixelwiseregression_amd import ops
+    n, g = 2 ** 20, 0.5
+    z = torch.tensor([0.0, 1.0], device=DEV).repeat(n, 1)
+    w = torch.ones(1, device=DEV, requires_grad=True)
+    r = ops.log_likelihood(z, torch.zeros(n, dtype=torch.long, device=DEV), w)
+    (gw,) = torch.autograd.grad(r.logp, w, torch.full((n,), g, device=DEV))
+    want = -n * g / (1 + math.exp(-1.0))
+    assert abs(gw.item() - want) <= (2 * (4 + 128) + 2) * 2.0 ** -24 * abs(want), (gw.item(), want)
