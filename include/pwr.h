@@ -400,7 +400,8 @@ int pwr_likelihood_fwd(const void* z, long long ldz, const float* w, int J, cons
                        float* logp, float* entropy, float* stats, float* top_logp, long long* top_index, long long rows, int V, int K, int dtype,
                        void* workspace, size_t workspace_bytes, void* stream);
 /* gz [rows][V] of `dtype` (contiguous) = the gradient of sum(glogp logp) + sum(gentropy entropy) with respect to z; glogp / gentropy [rows] or NULL
- * (zero); stats, entropy: from the forward pass.  gw [J] or NULL: the gradient with respect to w (rows a multiple of J); the workspace is for gw only. */
+ * (zero); stats, entropy: from the forward pass.  gw [J] or NULL: the gradient with respect to w (rows a multiple of J, J < 2^24); the workspace is for gw
+ * only. */
 size_t pwr_likelihood_bwd_workspace_bytes(long long rows, int V);
 int pwr_likelihood_bwd(const void* z, long long ldz, const float* w, int J, const float* mask, int mask_rows, const long long* index,
                        const float* stats, const float* entropy, const float* glogp, const float* gentropy, void* gz, float* gw, long long rows,

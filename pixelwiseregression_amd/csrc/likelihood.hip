@@ -738,7 +738,7 @@ extern "C" int pwr_likelihood_bwd(const void* z, long long ldz, const float* w, 
   if (dtype != PWR_F32 && dtype != PWR_BF16) return PWR_EINVAL;
   if (!like_countable(rows, V)) return PWR_EUNSUPPORTED;
   LikeBwdArgs a = {z, ldz, w, J, mask, mask_rows, index, stats, entropy, glogp, gentropy, gz, nullptr, rows, V, like_bwd_chunks(V)};
-  if (!like_fits(V <= kLikeWaveMax ? (rows + 3) / 4 : rows * a.chunks, 256)) return PWR_EUNSUPPORTED;
+  if (!like_fits(V <= kLikeWaveMax ? (rows + 3) / 4 : rows * a.chunks, 256) || (gw && !like_fits(J, 256))) return PWR_EUNSUPPORTED;
   if (gw) {
     if (rows && (!workspace || workspace_bytes < pwr_likelihood_bwd_workspace_bytes(rows, V))) return PWR_ENOSPACE;
     a.gw_part = (float*)workspace;

@@ -187,3 +187,8 @@ def test_the_barriers_of_one_workgroup_are_every_waves():
         else:
             head = token
     assert barriers >= 7
+
+
+def test_a_gradient_of_more_joints_than_a_launch_has_workgroups_is_refused():
+    bwd = lambda rows, J: _lib.lib().pwr_likelihood_bwd(SOME, 1, SOME, J, None, 1, None, SOME, SOME, None, None, SOME, SOME, rows, 1, 0, SOME, 2 ** 62, None)  # noqa: E731
+    assert bwd(2 ** 25, 2 ** 25) == EUNSUPPORTED and bwd(0, 2 ** 24) == EUNSUPPORTED
