@@ -221,16 +221,17 @@ def _likelihood_forward(r, topk, stats):
     return logp, entropy, top_logp, top_index, st
 
 
-def _likelihood_backward(r, stats, entropy, glogp, gentropy, need_w):
-    dev = r.z.device
-    gz = torch.empty(r.z.shape, device=dev, dtype=r.z.dtype)
+def _likelihood_backward(r, z, w, index, mask, stats, entropy, glogp, gentropy, need_w):
+    """(r: the numbers; the tensors as r had them)"""
+    dev = z.device
+    gz = torch.empty(z.shape, device=dev, dtype=z.dtype)
     gw = torch.empty(r.J, device=dev, dtype=torch.float32) if need_w else None
     glogp, gentropy = (_plain(g, torch.float32) if g is not None else None for g in (glogp, gentropy))
     l = _lib.lib()
     need = l.pwr_likelihood_bwd_workspace_bytes(r.rows, r.V) if need_w else 0
     ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     with _on(dev):
-        _lib.check(l.pwr_likelihood_bwd(r.z.data_ptr(), r.ld, _ptr(r.w), r.J, _ptr(r.mask), r.mask_rows, _ptr(r.index), stats.data_ptr(),
+        _lib.check(l.pwr_likelihood_bwd(z.data_ptr(), r.ld, _ptr(w), r.J, _ptr(mask), r.mask_rows, _ptr(index), stats.data_ptr(),
                                         entropy.data_ptr(), _ptr(glogp), _ptr(gentropy), gz.data_ptr(), _ptr(gw), r.rows, r.V, r.dtype, _ptr(ws), need,
                                         _lib.stream_ptr(dev)), "pwr_likelihood_bwd")
     return gz, gw
@@ -241,8 +242,14 @@ class LogLikelihoodFn(torch.autograd.Function):
     def forward(ctx, z, w, index, mask, topk):
         r = _Rows(z, index, w, mask)
         logp, entropy, top_logp, top_index, stats = _likelihood_forward(r, topk, True)
-        ctx.save_for_backward(z, w, index, mask, stats, entropy)     # (the inputs: so that a change of one before the backward pass is noticed)
-        ctx.r = r                                        # inputs and copies of inputs only: no cycle through an output
+        # The inputs, so that a change of one before the backward pass is noticed, and what the kernels read in their place: all of it saved, none held by
+        # ctx, so that the backward pass frees it, whoever keeps a result.
+        own = [t for t, given in ((r.z, z), (r.w, w), (r.index, index), (r.mask, mask)) if t is not given]
+        if own:
+            ctx.own = (r.z is not z, r.w is not w, r.index is not index, r.mask is not mask)
+        ctx.save_for_backward(z, w, index, mask, stats, entropy, *own)
+        r.z = r.w = r.index = r.mask = None
+        ctx.r = r
         ctx.set_materialize_grads(False)
         if topk:
             ctx.mark_non_differentiable(top_logp, top_index)
@@ -251,11 +258,14 @@ class LogLikelihoodFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, glogp, gentropy, _, __):
-        z, w, _, _, stats, entropy = ctx.saved_tensors
+        z, w, index, mask, stats, entropy, *own = ctx.saved_tensors
         if glogp is None and gentropy is None:
             return None, None, None, None, None
         need_z, need_w = ctx.needs_input_grad[:2]
-        gz, gw = _likelihood_backward(ctx.r, stats, entropy, glogp, gentropy, need_w)
+        read = [z, w, index, mask]
+        if own:
+            read = [own.pop(0) if apart else t for t, apart in zip(read, ctx.own)]
+        gz, gw = _likelihood_backward(ctx.r, *read, stats, entropy, glogp, gentropy, need_w)
         if gw is not None and (gw.shape != w.shape or gw.dtype != w.dtype):
             gw = gw.view(w.shape).to(w.dtype)
         return (gz if gz.shape == z.shape else gz.view(z.shape)) if need_z else None, gw, None, None, None
@@ -298,7 +308,7 @@ def likelihood_gradients(z, index, w, glogp, gentropy, mask=None):
                 raise ValueError("an upstream gradient must be %s, got %s" % (r.lead, tuple(g.shape)))
         _same_device(z, glogp, gentropy)
         logp, entropy, _, _, stats = _likelihood_forward(r, 0, True)
-        gz, gw = _likelihood_backward(r, stats, entropy, glogp, gentropy, w is not None)
+        gz, gw = _likelihood_backward(r, r.z, r.w, r.index, r.mask, stats, entropy, glogp, gentropy, w is not None)
     return LogLikelihood(logp, entropy, None, None), gz.view(z.shape), gw
 
 

@@ -131,3 +131,30 @@ def test_the_gradient_of_w_over_many_rows():
     (gw,) = torch.autograd.grad(r.logp, w, torch.full((n,), g, device=DEV))
     want = -n * g / (1 + math.exp(-1.0))
     assert abs(gw.item() - want) <= (2 * (4 + 128) + 2) * 2.0 ** -24 * abs(want), (gw.item(), want)
+
+
+@pytest.mark.parametrize("shape", [(64, 4, 64, 64), (64, 4, 4096), (256, 4096)])
+def test_a_kept_loss_does_not_keep_the_logits(shape):
+    """After the backward pass the logits are freed, whatever is left of the graph: a log of losses must not hold every step's maps."""
+    from pixelwiseregression_amd import ops
+    lead = shape[:1] if len(shape) == 2 else shape[:2]
+    index = torch.zeros(lead, dtype=torch.int32, device=DEV)             # (copied for the kernels, like the mask)
+    mask = torch.ones((shape[0], 1) + shape[2:] if len(shape) > 2 else shape, dtype=torch.bool, device=DEV)
+    scale = torch.ones((), device=DEV, requires_grad=True)
+    base = torch.randn(shape, device=DEV)
+    size = base.numel() * 4
+
+    def step():
+        r = ops.log_likelihood(base * scale, index, None, mask)
+        loss = r.logp.mean() + r.entropy.mean()
+        loss.backward(retain_graph=True)
+        loss.backward()
+        with pytest.raises(RuntimeError, match="second time"):
+            loss.backward()
+        return loss
+
+    step()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    kept = [step() for _ in range(4)]
+    assert torch.cuda.memory_allocated() - before < size // 2 and all(k.grad_fn is not None for k in kept)
