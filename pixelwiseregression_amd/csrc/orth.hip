@@ -5,8 +5,10 @@
 // five steps bring everything above ~1e-3 of the norm into about 0.7 .. 1.2, i.e. X is near the closest orthogonal matrix U V^T.  A matrix with
 // more rows than columns is worked on transposed, so A and B are as small as they can be: m x m with m = min(rows, cols), n = max.
 //
-// Numbers.  Everything between the products is kept as a PAIR of fp16, hi + lo = 22 bits, scaled by 4096 (|X| <= ~1.2, |A| <= ~1.5, |B| <= ~4
-// with the coefficients above; others are refused where an entry could reach 16, the end of fp16, and the low halves of entries down to 1e-5 are still normal fp16).  The matrix cores multiply fp16 pairs exactly and add in fp32.
+// Numbers.  Everything between the products is kept as a PAIR of fp16, hi + lo = 22 bits, scaled by 4096 (|X| <= ~1.2, |A| <= ~1.5, |B| <= ~3
+// with the coefficients above; others are refused where an entry could reach 16, the end of fp16).  Below 2^-14 = 6e-5 the low half is no normal fp16 any
+// more, and an entry is kept to 2^-37 instead of 2^-23 of itself: the result is right in norm, and a row that is 1e-5 of the others right to 1e-4 of
+// itself (in fp32 arithmetic: 2e-7).  The matrix cores multiply fp16 pairs exactly and add in fp32.
 //   fp32 tensors:  hi hi + hi lo + lo hi  -- three products per product; what is left out is 2^-22 of an entry, as much as an fp32 sum of this
 //                  length loses anyway (1e-6 of the result on the sizes tested, the same as fp32 products).
 //   bf16 tensors:  hi hi only -- one product -- but X itself advances from its 22 bits (the a X term), because noise put into X is amplified

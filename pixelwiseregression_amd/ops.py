@@ -345,7 +345,11 @@ def _written(*ts):
 def orthogonalize(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out=None):
     """The matrices ``x`` (``[..., rows, cols]``, float32 or bfloat16) made nearly orthogonal by ``steps`` Newton-Schulz products:
     ``X = x / (|x| + eps)``, then ``X = a X + (b A + c A A) X`` with ``A = X X^T`` (of the shorter side).  With the default coefficients every singular
-    value above about 1e-3 of the norm ends up between 0.7 and 1.2.  Float32: the precision of float32 products; bfloat16: 2e-3 of the result.
+    value above about 1e-3 of the norm ends up between 0.7 and 1.2.
+
+    Precision, in norm.  Float32: that of float32 products, for entries of ``x / (|x| + eps)`` above 6e-5; smaller ones are kept to 2^-37, so a row of
+    1e-5 times the others' size comes out right to 1e-4 of itself, and a matrix whose norm is 4e-4 eps to 4e-6.  Bfloat16: the products take 11 bits of
+    each entry, and the result is off by 2.0 - 2.5e-3 where rounding it alone costs 1.7e-3; ``orthogonalize(x.float()).to(x.dtype)`` has float32 products.
 
     Other coefficients are taken as far as no entry of X, A or ``b A + c A A`` can reach 16 (``a I`` included): ValueError where some matrix would.
 

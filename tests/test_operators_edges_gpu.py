@@ -158,3 +158,62 @@ def test_a_kept_loss_does_not_keep_the_logits(shape):
     before = torch.cuda.memory_allocated()
     kept = [step() for _ in range(4)]
     assert torch.cuda.memory_allocated() - before < size // 2 and all(k.grad_fn is not None for k in kept)
+
+
+def in_float32(x, steps=5, co=muon_ref.COEFFICIENTS, eps=1e-7):
+    """The iteration in float32 arithmetic throughout."""
+    a, b, c = (np.float32(v) for v in co)
+    if x.shape[0] > x.shape[1]:
+        return in_float32(x.T, steps, co, eps).T
+    y = (x / (np.sqrt((x * x).sum()) + eps)).astype(np.float32)
+    for _ in range(steps):
+        g = y @ y.T
+        y = a * y + (b * g + c * (g @ g)) @ y
+    return y.astype(np.float64)
+
+
+def kept(rows, m, n):
+    """What an absolute error of 2^-37 in every stored entry of X, A and B does to `rows` rows of an m x n result.  An error in X grows by at most a = 3.4445
+    a step; one in A gets into X by b + 2 c |A|, one in B as it is, both times |X| <= 1.21: 14.2 together.  Sums of a^5 ... a and of a^4 ... 1."""
+    return 2.0 ** -37 * math.sqrt(rows) * (682 * math.sqrt(n) + 198 * 14.2 * math.sqrt(m))
+
+
+@pytest.mark.parametrize("rows,cols", [(48, 400), (30, 1000), (128, 1152), (512, 130), (260, 900), (800, 5200)])
+@pytest.mark.parametrize("kind", ["gauss", "gradient", "lowrank", "decay"])
+def test_against_float32_products(rows, cols, kind):
+    """float32 tensors: three times as far from float64 as float32 products are (sums in another order, 22 bits for 24), plus the first rounding."""
+    from pixelwiseregression_amd import ops
+    r = np.random.default_rng(21)
+    m, n = sorted((rows, cols))
+    x = r.standard_normal((rows, cols))
+    if kind == "gradient":                                    # a few strong directions over noise
+        x = 1e-3 * ((r.standard_normal((rows, 8)) / np.arange(1, 9)) @ r.standard_normal((8, cols)) + x)
+    elif kind == "lowrank":
+        x = r.standard_normal((rows, m // 8)) @ r.standard_normal((m // 8, cols))
+    elif kind == "decay":                                     # singular values over four decades
+        u, _ = np.linalg.qr(r.standard_normal((rows, m)))
+        v, _ = np.linalg.qr(r.standard_normal((cols, m)))
+        x = (u * np.exp(-9.2 * np.arange(m) / m)) @ v.T
+    x = x.astype(np.float32).astype(np.float64)
+    got = ops.orthogonalize(torch.from_numpy(x).float().to(DEV)).cpu().double().numpy()
+    ref = muon_ref.newton_schulz(x)
+    assert np.linalg.norm(got - ref) <= 3 * np.linalg.norm(in_float32(x) - ref) + 2.0 ** -22 * np.linalg.norm(ref) + kept(m, m, n)
+
+
+@pytest.mark.parametrize("rows,cols", [(48, 400), (128, 1152), (512, 130), (260, 900), (800, 5200)])
+def test_rows_of_very_different_size(rows, cols):
+    """Each block of rows (of the shorter side) against float32 products and what entries below 2^-14 are kept to."""
+    from pixelwiseregression_amd import ops
+    r = np.random.default_rng(rows)
+    m, n = sorted((rows, cols))
+    scale = np.array([1.0, 1e-3, 1e-5, 1e-6])[np.arange(m) % 4]
+    x = r.standard_normal((m, n)) * scale[:, None]
+    x = (x if rows <= cols else x.T).astype(np.float32).astype(np.float64)
+    got = ops.orthogonalize(torch.from_numpy(x).float().to(DEV)).cpu().double().numpy()
+    ref, f32 = muon_ref.newton_schulz(x), in_float32(x)
+    if rows > cols:
+        got, ref, f32 = got.T, ref.T, f32.T
+    for k in range(4):
+        block = slice(k, None, 4)
+        err, size = np.linalg.norm((got - ref)[block]), np.linalg.norm(ref[block])
+        assert err <= 3 * np.linalg.norm((f32 - ref)[block]) + 2.0 ** -22 * size + kept(m / 4, m, n), (k, err / size)
