@@ -536,7 +536,7 @@ __global__ __launch_bounds__(256 * KG, KG > 1 ? 1 : TILE == 64 ? 4 : 2) void ort
   constexpr int SUMS = KG > 1 ? KG * TILE * TILE * 4 : 0;               // the groups' sums
   __shared__ __attribute__((aligned(16))) char lds[STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS];
   int t = blockIdx.x, part = 0;
-  const bool split_k = TILE == 128 && t >= g.whole;
+  const bool split_k = TILE == 128 && KIND != kApply && t >= g.whole;
   if (TILE == 128 && KIND != kApply) {
     // a die's workgroups: the same share of K of all tiles (parts in eighths), else neighbouring tiles
     if (split_k && !(g.parts & 7)) { const int v = t - g.whole; part = v % g.parts; t = g.whole + v / g.parts; }
@@ -790,7 +790,6 @@ __global__ __launch_bounds__(256 * KG, KG > 1 ? 1 : TILE == 64 ? 4 : 2) void ort
   }
 }
 
-// the split tiles of a product: a workgroup adds the parts of one of a tile's four fragment rows and finishes it
 // the shared 64 x 64 tiles of A: the workgroup of a tile's first share adds all of them
 template <int TERMS>
 __global__ __launch_bounds__(1024) void orth_join_shared_kernel(OrthArgs g) {
@@ -810,13 +809,14 @@ __global__ __launch_bounds__(1024) void orth_join_shared_kernel(OrthArgs g) {
   if (ti != tj) orth_mirror<kGram, 4>(g, o, w, i, j, d);
 }
 
-template <int TERMS, int KIND, typename OUT>
-__global__ __launch_bounds__(256) void orth_join_kernel(OrthArgs g, OUT fin, int last) {
+// the split 128 x 128 tiles of A or A A: a workgroup adds the parts of one of a tile's four fragment rows and finishes it
+template <int TERMS, int KIND>
+__global__ __launch_bounds__(256) void orth_join_kernel(OrthArgs g) {
   const int t = blockIdx.x >> 2, q = blockIdx.x & 3, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   int tile, ti, tj; int4 entry;
   const OrthItem o = orth_item(g, g.whole + t, tile, entry);
   const OrthWs w(o.Mp, o.Np);
-  orth_place(KIND != kApply, tile, entry, o.Mp / 128, o.Np / 128, 1, ti, tj);
+  orth_place(true, tile, entry, o.Mp / 128, o.Np / 128, 1, ti, tj);
   const int i = ti * 128 + (wid >> 1) * 64 + 16 * q + (lane & 15), j = tj * 128 + (wid & 1) * 64 + 16 * (lane >> 4);
   const OrthPair<16> beside = orth_beside<KIND, 16>(g, o, w, i, j);
   const f32x4* s = g.slab + (long long)t * g.parts * 4096 + q * 256 + tid;
@@ -829,8 +829,8 @@ __global__ __launch_bounds__(256) void orth_join_kernel(OrthArgs g, OUT fin, int
   float v[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) v[e] = a[e / 4][e % 4];
-  const OrthPair<16> d = orth_finish<TERMS, KIND, 16, OUT>(g, o, w, fin, last, i, j, v, beside);
-  if (KIND != kApply && ti != tj) orth_mirror<KIND, 16>(g, o, w, i, j, d);
+  const OrthPair<16> d = orth_finish<TERMS, KIND, 16, OrthNone>(g, o, w, OrthNone{}, 0, i, j, v, beside);
+  if (ti != tj) orth_mirror<KIND, 16>(g, o, w, i, j, d);
 }
 
 // ---- small matrices: one workgroup of eight waves does a whole matrix, X in LDS for all steps.  MT x 16 rows (m <= 32 or 64), up to NCAP columns.
@@ -1205,7 +1205,7 @@ static int orth_run(const OrthArgs& g, const OrthCounts& n, const int4* const (&
     }
     if constexpr (TILE == 128) {
       if (h.whole < n.n[2])
-        hipLaunchKernelGGL((orth_join_kernel<TERMS, KIND, OrthNone>), dim3((unsigned)(4 * (n.n[2] - h.whole))), b, 0, s, h, OrthNone{}, 0);
+        hipLaunchKernelGGL((orth_join_kernel<TERMS, KIND>), dim3((unsigned)(4 * (n.n[2] - h.whole))), b, 0, s, h);
     }
   };
   for (int k = 0; k < steps; ++k) {
