@@ -652,8 +652,11 @@ static bool like_fits(long long blocks, int threads) { return blocks <= 0xffffff
 // what the kernels count in 32 bits (and no product of the checks below leaves 64)
 static bool like_countable(long long rows, int V) { return rows <= 0xffffffffll && V <= kLikeMaxRow; }
 
+// rows that one workgroup each walks
+static bool like_walks(long long rows, int V, int K) { return !K && V > 4096 && (rows >= kLikeWalkRows || like_chunks(rows, V, K) == 1); }
+
 extern "C" size_t pwr_likelihood_workspace_bytes(long long rows, int V, int K) {
-  if (rows <= 0 || V <= 0 || K < 0 || !like_countable(rows, V)) return 0;
+  if (rows <= 0 || V <= 0 || K < 0 || !like_countable(rows, V) || like_walks(rows, V, K)) return 0;
   const int n = like_chunks(rows, V, K);
   return n == 1 ? 0 : (size_t)rows * n * (16 + 8 * (size_t)K);
 }
@@ -670,7 +673,7 @@ static int like_forward(const LikeArgs& a, hipStream_t s) {
   }
   constexpr int N = 16 / sizeof(T);
   if constexpr (!TOP) {
-    if (a.V > 4096 && (rows >= kLikeWalkRows || a.chunks == 1)) {
+    if (like_walks(rows, a.V, 0)) {
       if (!like_fits(rows, 256)) return PWR_EUNSUPPORTED;
       hipLaunchKernelGGL((like_walk_kernel<T, 256, 16>), dim3((unsigned)rows), dim3(256), 0, s, a);
       return (int)hipGetLastError();
@@ -701,8 +704,9 @@ extern "C" int pwr_likelihood_fwd(const void* z, long long ldz, const float* w, 
   if (dtype != PWR_F32 && dtype != PWR_BF16) return PWR_EINVAL;
   LikeArgs a = {z, ldz, w, J, mask, mask_rows, index, rows, V, K, logp, entropy, stats, top_logp, top_index, 1, V, nullptr, nullptr, nullptr};
   if (K > kLikeMaxTop || !like_countable(rows, V)) return PWR_EUNSUPPORTED;
-  a.chunk = like_chunk(rows, V, K);
-  a.chunks = like_chunks(rows, V, K);
+  const bool walks = like_walks(rows, V, K);
+  a.chunk = walks ? V : like_chunk(rows, V, K);
+  a.chunks = walks ? 1 : like_chunks(rows, V, K);
   if ((long long)a.chunks * K > kLikeJoin || rows * a.chunks > 0x7fffffffll) return PWR_EUNSUPPORTED;
   if (a.chunks > 1) {
     if (!workspace || workspace_bytes < pwr_likelihood_workspace_bytes(rows, V, K)) return PWR_ENOSPACE;

@@ -192,3 +192,13 @@ def test_the_barriers_of_one_workgroup_are_every_waves():
 def test_a_gradient_of_more_joints_than_a_launch_has_workgroups_is_refused():
     bwd = lambda rows, J: _lib.lib().pwr_likelihood_bwd(SOME, 1, SOME, J, None, 1, None, SOME, SOME, None, None, SOME, SOME, rows, 1, 0, SOME, 2 ** 62, None)  # noqa: E731
     assert bwd(2 ** 25, 2 ** 25) == EUNSUPPORTED and bwd(0, 2 ** 24) == EUNSUPPORTED
+
+
+def test_rows_that_are_walked_need_no_workspace():
+    """512 long rows and more without alternatives go to a workgroup each; fewer are split, and joined from a workspace."""
+    l = _lib.lib()
+    assert l.pwr_likelihood_workspace_bytes(512, 100000, 0) == 0 and l.pwr_likelihood_workspace_bytes(4096, 50001, 0) == 0
+    assert l.pwr_likelihood_workspace_bytes(511, 100000, 0) == 511 * 7 * 16 and l.pwr_likelihood_workspace_bytes(512, 100000, 1) == 512 * 7 * (16 + 8)
+    assert l.pwr_likelihood_fwd(SOME, 0, None, 1, None, 1, None, None, SOME, None, None, None, 511, 100000, 0, 0, None, 0, None) == -3
+    # (refused by the number of its threads, a workgroup of 256 a row: the last check)
+    assert l.pwr_likelihood_fwd(SOME, 0, None, 1, None, 1, None, None, SOME, None, None, None, 2 ** 24, 100000, 0, 0, None, 0, None) == EUNSUPPORTED
