@@ -217,3 +217,75 @@ def test_rows_of_very_different_size(rows, cols):
         block = slice(k, None, 4)
         err, size = np.linalg.norm((got - ref)[block]), np.linalg.norm(ref[block])
         assert err <= 3 * np.linalg.norm((f32 - ref)[block]) + 2.0 ** -22 * size + kept(m / 4, m, n), (k, err / size)
+
+
+@pytest.mark.parametrize("shape,dtype", [((6, 4, 700), torch.float32), ((6, 4, 9000), torch.bfloat16), ((5, 3, 16, 16), torch.float32), ((520, 5000), torch.bfloat16),
+                                         ((7, 40), torch.float32), ((0, 4, 50), torch.float32)])
+@pytest.mark.parametrize("with_w", [False, True])
+@pytest.mark.parametrize("mask", [None, "sample", "row"])
+def test_likelihood_gradients_are_those_of_autograd(shape, dtype, with_w, mask):
+    """The same kernels on the same rows: the same bits as log_likelihood and its backward pass, whichever gradients are given."""
+    from pixelwiseregression_amd import ops
+    g = torch.Generator().manual_seed(4)
+    lead, J = (shape[:1], 1) if len(shape) == 2 else (shape[:2], shape[1])
+    V = shape[-1] if len(shape) < 4 else shape[2] * shape[3]
+    z = (3 * torch.randn(shape, generator=g)).to(dtype).to(DEV)
+    index = torch.randint(-1, V, lead, generator=g).to(DEV)
+    w = (0.5 + torch.rand(J, 1, generator=g)).to(DEV) if with_w else None
+    m = None
+    if mask is not None:
+        m = torch.rand((shape[0],) + (((1,) if mask == "sample" else shape[1:2]) if len(shape) > 2 else ()) + shape[len(lead):], generator=g) < 0.5
+        m[:1] = False                                         # a map without a pixel
+        m = m.to(DEV)
+    gl, ge = (torch.randn(lead, generator=g).to(DEV) for _ in range(2))
+    for up in ((gl, ge), (gl, None), (None, ge), (None, None)):
+        r, gz, gw = ops.likelihood_gradients(z, index, w, *up, mask=m)
+        leaves = [z.detach().requires_grad_()] + ([w.detach().requires_grad_()] if with_w else [])
+        q = ops.log_likelihood(leaves[0], index, leaves[1] if with_w else None, m)
+        assert torch.equal(r.logp, q.logp) and torch.equal(r.entropy, q.entropy) and r.top_logp is None and r.top_index is None
+        assert not r.logp.requires_grad and gz.shape == z.shape and gz.dtype == z.dtype and (gw is None) == (not with_w)
+        if up == (None, None):
+            assert (gz == 0).all() and (gw is None or (gw == 0).all())
+            continue
+        outs = [(o, u) for o, u in zip((q.logp, q.entropy), up) if u is not None]
+        want = torch.autograd.grad([o for o, _ in outs], leaves, [u for _, u in outs])
+        assert torch.equal(gz, want[0])
+        if with_w:
+            assert gw.shape == (J,) and torch.equal(gw, want[1].view(J))
+    with pytest.raises(ValueError, match="upstream"):
+        ops.likelihood_gradients(z, index, w, gl[..., None], ge, mask=m)
+
+
+@pytest.mark.parametrize("precision", ["bf16", "fp32"])
+def test_the_likelihood_terms_of_a_training_step_in_both_precisions(precision):
+    """The loss of TrainStep(lambda_nll, lambda_entropy) is that of the maps the same forward pass returns, and the terms reach the parameters like the same
+    terms through autograd.  The logits are fp32 in both: their gradients agree to (4 S + 128) 2^-24.  In bf16 the two backward passes round gradients
+    that differ by that much, and a rounding that falls the other way is a whole step, 2^-8: at most 2^-8 of the norm for each of the
+    dozen layers between the heads and the stem of this network, if all of them fell so, and twice that behind the norms' subtractions."""
+    from pixelwiseregression_amd import PixelwiseRegression, ops
+    from pixelwiseregression_amd.synthetic import make_batch
+    from pixelwiseregression_amd.train import TrainStep
+    torch.manual_seed(0)
+    B, J, P = 3, 4, 16
+    m = PixelwiseRegression(J, stage=2, label_size=P, features=32, level=2, norm_method="instance").to(DEV).set_precision(precision).train()
+    b = {k: v.to(DEV) for k, v in make_batch(B, J, S=2 * P, seed=2).items()}
+    args = (b["img"], b["label_img"], b["mask"], b["uvd"])
+    plain = TrainStep(m, opt="sgd", lr=0.0)(*args).item()
+    base = m.flat_grad().clone()
+    loss = TrainStep(m, opt="sgd", lr=0.0, lambda_nll=0.3, lambda_entropy=0.05)(*args).item()
+    grad = m.flat_grad().clone()
+    for p in m.parameters():
+        p.grad = None
+    index = ops.heatmap_pixels(b["uvd"], P)
+    want = 0.0
+    for heat, _, uvd in m(*args[:3]):
+        logs = heat.double().flatten(2).log()
+        logp = logs.gather(2, index.clamp(min=0)[..., None])[..., 0] * (index >= 0)
+        want = want + torch.mean(torch.sum((uvd - b["uvd"]) ** 2, dim=2)) - 0.3 * logp.mean() + 0.05 * -(heat.flatten(2) * logs).sum(-1).mean()
+    want.backward()
+    auto = m.flat_grad()
+    assert abs(loss - want.item()) <= 1e-5 * abs(want.item()) and abs(loss - plain) > 0.1
+    assert (grad - base).norm() > 0.01 * base.norm()
+    assert (grad - auto).norm() <= (1e-3 if precision == "fp32" else 24 * 2.0 ** -8) * auto.norm(), ((grad - auto).norm() / auto.norm()).item()
+    for o in [o for n, (o, _) in m._offsets.items() if n.endswith(".w")]:         # the temperature's: fp32 all the way
+        assert (grad[o:o + J] - auto[o:o + J]).norm() <= 1e-3 * auto[o:o + J].norm()
