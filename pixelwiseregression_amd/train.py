@@ -127,8 +127,11 @@ class TrainStep:
             _lib.check(l.pwr_adamw_step(flat.data_ptr(), grad.data_ptr(), self.m.data_ptr(), self.v.data_ptr(), n, self.lr, self.beta1,
                                         self.beta2, self.eps, self.wd, self.steps, scale, stream), "pwr_adamw_step")
         elif self.opt == "muon":
-            self.muon.flat, self.muon.lr, self.muon.weight_decay, self.muon.steps = flat, self.lr, self.wd, self.steps - 1
-            self.muon.step(grad, scale)
+            u = self.muon                                    # (what the other two read here too: a state or a rate set between steps counts)
+            u.flat, u.lr, u.weight_decay, u.steps = flat, self.lr, self.wd, self.steps - 1
+            u.beta1, u.beta2, u.adam_eps = self.beta1, self.beta2, self.eps
+            u.buf, u.v = u._check(self.m, "m"), u._check(self.v, "v")
+            u.step(grad, scale)
         else:
             _lib.check(l.pwr_sgd_step(flat.data_ptr(), grad.data_ptr(), self.m.data_ptr(), n, self.lr, self.beta1, self.wd,
                                       1 if self.steps == 1 else 0, scale, stream), "pwr_sgd_step")

@@ -289,3 +289,26 @@ def test_the_likelihood_terms_of_a_training_step_in_both_precisions(precision):
     assert (grad - auto).norm() <= (1e-3 if precision == "fp32" else 24 * 2.0 ** -8) * auto.norm(), ((grad - auto).norm() / auto.norm()).item()
     for o in [o for n, (o, _) in m._offsets.items() if n.endswith(".w")]:         # the temperature's: fp32 all the way
         assert (grad[o:o + J] - auto[o:o + J]).norm() <= 1e-3 * auto[o:o + J].norm()
+
+
+def test_a_state_set_between_training_steps_counts():
+    """TrainStep's moments, rates and betas are its attributes, whatever the optimizer: a resumed state is what the next step goes on from."""
+    from pixelwiseregression_amd import PixelwiseRegression, optim
+    from pixelwiseregression_amd.synthetic import make_batch
+    from pixelwiseregression_amd.train import TrainStep
+    torch.manual_seed(0)
+    m = PixelwiseRegression(4, stage=1, label_size=16, features=32, level=1, norm_method="instance").to(DEV).train()
+    b = {k: v.to(DEV) for k, v in make_batch(2, 4, S=32, seed=2).items()}
+    ts = TrainStep(m, opt="muon", lr=2e-3)
+    n = m.flat_parameters().numel()
+    ts.m, ts.v, ts.steps = 1e-3 * torch.randn(n, device=DEV), 1e-6 * torch.rand(n, device=DEV), 6
+    ts.beta1, ts.beta2, ts.eps, ts.wd, ts.lr = 0.8, 0.99, 1e-6, 0.02, 1e-3
+    p, buf, v = m.flat_parameters().clone(), ts.m.clone(), ts.v.clone()
+    ts(b["img"], b["label_img"], b["mask"], b["uvd"])
+    twin = optim.Muon(p, [s for _, s in m._offsets.values()], lr=1e-3, weight_decay=0.02, beta1=0.8, beta2=0.99, adam_eps=1e-6, buf=buf, v=v)
+    twin.steps = 6
+    twin.step(m.flat_grad())
+    assert torch.equal(p, m.flat_parameters()) and torch.equal(buf, ts.m) and torch.equal(v, ts.v) and ts.steps == 7
+    ts.m = ts.m[1:]
+    with pytest.raises(Exception):
+        ts(b["img"], b["label_img"], b["mask"], b["uvd"])
