@@ -312,3 +312,29 @@ def test_a_state_set_between_training_steps_counts():
     ts.m = ts.m[1:]
     with pytest.raises(Exception):
         ts(b["img"], b["label_img"], b["mask"], b["uvd"])
+
+
+@pytest.mark.parametrize("V", [30, 900, 6000])
+def test_a_w_of_any_sign_and_size(V):
+    """w < 0, w = 0 (every allowed pixel alike) and a w that leaves nothing of the logits' differences, against float64.  The bound is that of
+    test_likelihood_gpu.py: (4 S + 128) 2^-24 of a probability, S = max |w z|, and 2 x that of the terms of a gradient."""
+    from pixelwiseregression_amd import ops
+    g = torch.Generator().manual_seed(V)
+    z, index = 3 * torch.randn(3, 4, V, generator=g), torch.randint(0, V, (3, 4), generator=g)
+    w = torch.tensor([-1.7, 0.0, 1e-30, -0.01])
+    mask = torch.ones(3, 1, V)
+    mask[1, 0, ::2] = 0
+    gl, ge = (torch.randn(3, 4, generator=g) for _ in range(2))
+    r, gz, gw = ops.likelihood_gradients(*(t.to(DEV) for t in (z, index, w, gl, ge)), mask=mask.to(DEV))
+    ref = likelihood_ref.rows(z.numpy(), index.numpy(), w.numpy(), np.broadcast_to(mask.numpy(), z.shape), 0, gl.numpy(), ge.numpy())
+    aw = np.abs(w.double().numpy())
+    tol = (4 * aw * np.abs(z.numpy()).max() + 128) * 2.0 ** -24
+    host = lambda t: t.cpu().double().numpy()  # noqa: E731
+    fin = np.isfinite(ref["logp"])
+    assert (np.isfinite(host(r.logp)) == fin).all() and (np.abs(host(r.logp) - ref["logp"])[fin] <= np.broadcast_to(tol, fin.shape)[fin]).all()
+    assert (np.abs(host(r.entropy) - ref["entropy"]) <= (1 + ref["entropy"]) * tol).all()
+    p, lp, H = ref["p"], np.where(ref["p"] > 0, ref["logs"], 0.0), ref["entropy"][..., None]
+    size = (np.abs(gl.numpy())[..., None] * p + np.abs(ge.numpy())[..., None] * p * (np.abs(lp) + H + 1)) * 2 * tol[:, None] + 2.0 ** -126
+    assert (np.abs(host(gz) - ref["gz"]) <= size * aw[:, None] + 4 * 2.0 ** -24 * np.abs(ref["gz"])).all()
+    given = np.abs(gl.numpy()) * np.abs(z.numpy()).max()
+    assert (np.abs(host(gw) - ref["gw"]) <= (size * 2 * np.abs(z.numpy()).max()).sum((0, 2)) + 160 * 2.0 ** -24 * given.sum(0)).all()
