@@ -1334,7 +1334,9 @@ struct MuonHead {
 };
 constexpr unsigned long long kMuonMagic = 0x32304e4f554d5750ull;
 
-// a list is worked on in the tile that most of its products want (in units of a 64 x 64 x 64 block), after orth_tile, padding aside
+// A list is worked on in the tile that most of its products want (in units of a 64 x 64 x 64 block), after orth_tile, padding aside.  A step in 128 / 64:
+// 4 of 2048 x 2048 2347 / 3673 us, 12 of 1024 x 4096 3241 / 4143, 12 of 1024 x 1024 1106 / 1397, 4 of 768 x 3000 690 / 747; half of the work in one
+// 2048 x 2048, the rest in 60 of 256 x 2304, 2053 / 1982; a list of 1000 x 2100, 2500 x 900, 1000 x 1000 and small ones 644 / 620.
 int muon_tile(const std::vector<OrthItem>& v) {
   double wide = 0, all = 0;
   long long tiles = 0;
