@@ -421,13 +421,13 @@ __global__ __launch_bounds__(256) void like_join_kernel(LikeArgs a) {
   float M = -INFINITY;
   for (int c = lane; c < a.chunks; c += 64) M = fmaxf(M, part[c].x);
   M = wave_max(M);
-  LikeStat st = {M, 0.f, 0.f, 0.f};
+  double tc = 0.0, tr = 0.0, tq = 0.0;                              // (a row may have 2^17 pieces, 2048 a lane)
   for (int c = lane; c < a.chunks; c += 64) {
     const f32x4 v = part[c];
     const LikeStat x = like_shift(LikeStat{v.x, v.y, v.z, v.w}, M);
-    st.c += x.c; st.r += x.r; st.q += x.q;
+    tc += x.c; tr += x.r; tq += x.q;
   }
-  st.c = wave_sum(st.c); st.r = wave_sum(st.r); st.q = wave_sum(st.q);
+  const LikeStat st = {M, wave_sum((float)tc), wave_sum((float)tr), wave_sum((float)tq)};
   const float lt = like_log_total(st);
   if (tid == 255) like_finish(a, row, st, lt, given);
   if (!a.K) return;

@@ -338,3 +338,18 @@ def test_a_w_of_any_sign_and_size(V):
     assert (np.abs(host(gz) - ref["gz"]) <= size * aw[:, None] + 4 * 2.0 ** -24 * np.abs(ref["gz"])).all()
     given = np.abs(gl.numpy()) * np.abs(z.numpy()).max()
     assert (np.abs(host(gw) - ref["gw"]) <= (size * 2 * np.abs(z.numpy()).max()).sum((0, 2)) + 160 * 2.0 ** -24 * given.sum(0)).all()
+
+
+def test_one_very_long_row():
+    """2^30 logits in 65536 pieces: equal ones but for the first.  log p of the second is d - log(1 + (V - 1) e^d); the tolerance of test_likelihood_gpu.py
+    with S = |d|, which has room for the last rounding of a number near 21.  (One after another, a lane's 1024 pieces lose 249 2^-24 of the sum.)"""
+    from pixelwiseregression_amd import ops
+    V = 2 ** 30
+    z = torch.full((1, V), -0.75, device=DEV, dtype=torch.bfloat16)
+    d = z[0, 1].item()
+    z[0, 0] = 0.0
+    r = ops.log_likelihood(z, torch.tensor([1], device=DEV), topk=0)
+    log_total = math.log(1 + (V - 1) * math.exp(d))
+    entropy = log_total - (V - 1) * d * math.exp(d) / (1 + (V - 1) * math.exp(d))
+    tol = (4 * abs(d) + 128) * 2.0 ** -24
+    assert abs(r.logp.item() - (d - log_total)) <= tol and abs(r.entropy.item() - entropy) <= (1 + entropy) * tol
