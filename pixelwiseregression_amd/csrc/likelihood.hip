@@ -322,7 +322,7 @@ __global__ __launch_bounds__(NT) void like_fwd_kernel(LikeArgs a) {
 
 // Long rows, enough of them to fill the chip, without alternatives: one workgroup walks its row in parts of NT x VPT values, the next part's loads under
 // way while it works on one.  The sums are kept relative to the largest value so far, per thread; one barrier per part.  A part's sixteen values are added up
-// by themselves and the parts by compensated additions: the length of the row costs no bits, a new maximum one rounding.  4096 rows of 50001 bf16: 256 threads
+// by themselves and the parts by compensated additions: the length of the row costs no bits, a new maximum three roundings of what is there.  4096 rows of 50001 bf16: 256 threads
 // x 16 values 102 us = 4.0 TB/s (50000, rows that start aligned: 88 us = 4.7), 256 x 32 112, 512 x 16 128, 1024 x 16 189, a workgroup per chunk and a
 // join 161; 5376 rows of 16384 fp32: 64 us = 5.5 TB/s against 74 in one piece.
 template <typename T, int NT, int VPT>

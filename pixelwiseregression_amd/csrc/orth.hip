@@ -1225,8 +1225,7 @@ constexpr long long kOrthMaxBlocks = 0xffffffffll / 1024;         // a launch ha
 // [-m, m], so the largest ones are followed exactly (0.2 % a step are left for the roundings); the last X is not stored.
 constexpr double kOrthLargest = 15.9;
 static double orth_quadratic(double k, double b, double c, double u) {         // max |k + b t + c t^2| over 0 <= t <= u
-  double m = std::max(fabs(k), fabs(k + u * (b + c * u)));
-  const double t = c != 0.0 ? -b / (2 * c) : -1.0;
+  const double m = std::max(fabs(k), fabs(k + u * (b + c * u))), t = -b / (2 * c);                 // (c = 0: no number in between)
   return t > 0.0 && t < u ? std::max(m, fabs(k + t * (b + c * t))) : m;
 }
 static bool orth_range_ok(int steps, double a, double b, double c) {
@@ -1237,10 +1236,11 @@ static bool orth_range_ok(int steps, double a, double b, double c) {
     if (!(u < kOrthLargest) || !(orth_quadratic(0.0, b, c, u) < kOrthLargest) || !(orth_quadratic(a, b, c, u) < kOrthLargest)) return false;
     auto next = [&](double t) { return sqrt(t) * fabs(a + t * (b + c * t)); };
     double m = next(u);
-    // where the map turns: a + 3 b t + 5 c t^2 = 0
-    const double disc = 9 * b * b - 20 * a * c, root = disc > 0.0 ? sqrt(disc) : 0.0;
-    for (const double t : {c != 0.0 ? (-3 * b + root) / (10 * c) : b != 0.0 ? -a / (3 * b) : -1.0, c != 0.0 ? (-3 * b - root) / (10 * c) : -1.0})
-      if (disc >= 0.0 && t > 0.0 && t < u) m = std::max(m, next(t));
+    // where the map turns: a + 3 b t + 5 c t^2 = 0 (its roots without a difference of near numbers, c = 0 included)
+    const double disc = 9 * b * b - 20 * a * c, q = -0.5 * (3 * b + (b < 0.0 ? -1.0 : 1.0) * sqrt(std::max(disc, 0.0)));
+    if (disc >= 0.0)
+      for (const double t : {q / (5 * c), a / q})
+        if (t > 0.0 && t < u) m = std::max(m, next(t));
     s = 1.002 * m;
   }
   return true;

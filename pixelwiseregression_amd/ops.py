@@ -115,7 +115,7 @@ def _dtype_tag(t, what):
 
 def _tangents(*ts):
     """Whether one of them carries a forward-mode tangent (requires_grad says nothing of those)."""
-    return forward_ad._current_level >= 0 and any(t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _same_device(t, *others):
@@ -278,8 +278,9 @@ def log_likelihood(z, index, w=None, mask=None, topk=0):
 
     z: logits ``[B, J, H, W]``, ``[B, J, V]`` or ``[N, V]``, float32 or bfloat16.  index: ``[B, J]`` (``[N]``) whole numbers, -1 where no pixel is
     given (log likelihood 0, no gradient); a pixel outside its map gives NaN; None: no ``logp``.  w: one number per joint.  mask: ``[B, 1, H, W]``
-    (one per sample) or one per map; 0 = not allowed, whatever z holds there.  topk <= 32 (less for maps of over 2^21 pixels): equal values go by the lowest index; what does not exist
-    (masked, -inf, beyond the map) is ``(-inf, -1)``.  A map without an allowed pixel: -inf, entropy 0, zero gradient.
+    (one per sample) or one per map; 0 = not allowed, whatever z holds there.  A map has 2^31 - 2^14 pixels at most.  topk <= 32 (less for maps of over
+    2^21 pixels): equal values go by the lowest index; what does not exist (masked, -inf, beyond the map) is ``(-inf, -1)``.  A map without an allowed
+    pixel: -inf, entropy 0, zero gradient.
 
     Returns ``LogLikelihood(logp, entropy, top_logp, top_index)``, float32 (int64 the last); gradients of ``logp`` and ``entropy`` reach z and w
     (reverse mode; a forward-mode tangent is refused).

@@ -102,7 +102,10 @@ def test_coefficients_that_leave_the_pairs_are_refused(anywhere):
     # linear maps and single steps: both sides of each limit
     for steps, co, ok in ((3, (1.98, 0.0, 0.0), 1), (3, (2.0, 0.0, 0.0), 0), (1, (1.0, -15.8, 0.0), 1), (1, (1.0, -16.0, 0.0), 0), (1, (15.8, -15.8, 0.0), 1),
                           (1, (16.0, -15.0, 0.0), 0), (2, (2.5, -0.06, 0.0), 1), (4, (2.5, -0.06, 0.0), 0), (5, (3.0, -0.065, 0.0), 0),
-                          (1, (math.nan, 0.0, 0.0), 0), (1, (0.0, math.inf, 0.0), 0)):
+                          (1, (math.nan, 0.0, 0.0), 0), (1, (0.0, math.inf, 0.0), 0),
+                          # the largest s between 0 and 1, whatever c is next to b, or b next to a c
+                          (2, (6.9, -6.9, 0.0), 0), (2, (6.9, -6.9, 1e-17), 0), (2, (6.9, -6.9, -1e-30), 0), (2, (9.0, 0.0, -9.0), 0), (2, (9.0, 1e-20, -9.0), 0),
+                          (2, (3.0, 1e-20, -3.0), 0), (2, (2.0, 1e-20, -2.0), 1), (64, (0.0, 0.0, 0.0), 1)):
         assert (l.pwr_orthogonalize_range(steps, *co) == 0) == bool(ok), (steps, co)
         if not ok:
             assert l.pwr_orthogonalize(SOME, 12, 4, SOME, 3, 4, 1, 0, steps, *co, 1e-7, SOME, 2 ** 40, None) == EUNSUPPORTED
