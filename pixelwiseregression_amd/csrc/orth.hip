@@ -1143,8 +1143,8 @@ static int orth_tile(int rows, int cols, long long batch) {
   return orth_cost(rows, cols, batch, 128) * 8192 <= orth_cost(rows, cols, batch, 64) * (8192.0 + m) ? 128 : 64;
 }
 
-// X of such a matrix fits the LDS of one CU.  In one workgroup a matrix / by launches: 64 x 128 fp32 24 / 78 us, 64 x 512 59 / 90, 32 x 1024 47 / 92,
-// 600 of 64 x 500 bf16 175 / 374, 2000 of 64 x 128 bf16 193 / 470.
+// X of such a matrix fits the LDS of one CU.  In one workgroup a matrix / by launches: 64 x 128 fp32 21 / 78 us, 64 x 512 46 / 90, 32 x 1024 38 / 92,
+// 600 of 64 x 500 bf16 142 / 374, 2000 of 64 x 128 bf16 165 / 470.
 static bool orth_is_small(int rows, int cols) {
   const long long m = std::min(rows, cols), n = (std::max(rows, cols) + 63ll) / 64 * 64;
   return m <= 32 ? n <= 1024 : m <= 64 && n <= 512;
